@@ -910,6 +910,105 @@ int n2_snapshot_read(n2_snapshot_t* snapshot, n2_stream_t stream, const n2_snaps
 void n2_snapshot_close(n2_snapshot_t* snapshot);
 
 /* ------------------------------------------------------------------------
+ * Layers of any width, beside the 64-wide fully fused networks: linear layers with bias, activation and residual
+ * (tcnn's CutlassMLP is what the reference's create_network, nerf_network.h:57 and :65, gives for other widths) and
+ * layer norm, forward and backward, and the norm of many tensors' gradients with clipping.
+ *
+ * Rows: a matrix of n rows and c columns has element (i, j) at i * stride + j (elements, stride >= c): one row per
+ * sample, unlike the SoA matrices above.  Rows need no alignment beyond their type's.  Sums, statistics and norms are
+ * held in fp32 or more whatever the type; what is stored is rounded once.
+ * No call touches what lies behind the last row or between a row's end and the next row.
+ * An output may be the same rows as the residual (d_output == d_residual with equal strides, also for d_dL_dskip and
+ * d_dL_dinput); any other overlap of what is written with what is read or written is refused.
+ * Every sum is formed in an order that follows from the sizes alone: two calls on the same inputs give the same bits.
+ * The workspaces are read only behind what the same call has written; calls that may run at the same time (also two
+ * captured graphs) need workspaces of their own.
+ * ---------------------------------------------------------------------- */
+typedef enum n2_dtype {
+	N2_DTYPE_F16 = 0,
+	N2_DTYPE_BF16 = 1,
+	N2_DTYPE_F32 = 2
+} n2_dtype;
+
+typedef enum n2_activation {
+	N2_ACTIVATION_NONE = 0,
+	N2_ACTIVATION_RELU = 1, /* max(z, 0); the gradient at 0 is 0; a z that is no number gives 0, as tcnn's comparison does */
+	N2_ACTIVATION_SILU = 2, /* z / (1 + exp(-z)) */
+	N2_ACTIVATION_GELU = 3  /* z * (1 + erf(z / sqrt(2))) / 2 */
+} n2_activation;
+
+/* y = act(z) + r, z = x W^T + b, for n_rows rows.  F16 or BF16, one type for all matrices.
+ *  d_weights         [out_width][in_width], row-major without padding
+ *  d_bias            NULL or [out_width]
+ *  d_residual        NULL or [n_rows][out_width]
+ *  d_pre_activation  NULL or [n_rows][out_width], written: z, what the backward pass of an activation reads
+ *  The activation is taken of z before it is rounded.  in_width and out_width are 1 to 65536.
+ *  d_workspace       n2_linear_forward_workspace_bytes(n_rows, in_width, out_width) bytes (may be 0), 16-byte aligned */
+uint64_t n2_linear_forward_workspace_bytes(uint32_t n_rows, uint32_t in_width, uint32_t out_width);
+int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation activation, uint32_t n_rows, uint32_t in_width, uint32_t out_width,
+                      const void* d_weights, const void* d_bias, const void* d_input, uint64_t input_stride, const void* d_residual,
+                      uint64_t residual_stride, void* d_output, uint64_t output_stride, void* d_pre_activation, uint64_t pre_stride,
+                      void* d_workspace, uint64_t workspace_bytes);
+
+/* dL/dz = dL/dy * act'(z);  dL/dx = dL/dz W;  dL/dW = dL/dz^T x;  db = column sums of dL/dz.  (The residual's gradient is
+ * dL/dy itself.)  dL/dz is rounded to the type before it meets the matrix cores; the column sums take it unrounded.
+ *  d_pre_activation  z as the forward pass left it; not read (may be NULL) for N2_ACTIVATION_NONE
+ *  d_dL_dinput       NULL or [n_rows][in_width], written
+ *  d_dL_dweights, d_dL_dbias   NULL or [out_width][in_width] and [out_width]: written (OVERWRITE), added to with one rounding
+ *                    (ACCUMULATE) or left alone (IGNORE).  Without rows OVERWRITE leaves zeros. */
+uint64_t n2_linear_backward_workspace_bytes(uint32_t n_rows, uint32_t in_width, uint32_t out_width);
+int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation activation, uint32_t n_rows, uint32_t in_width, uint32_t out_width,
+                       const void* d_weights, const void* d_input, uint64_t input_stride, const void* d_pre_activation, uint64_t pre_stride,
+                       const void* d_dL_doutput, uint64_t dL_doutput_stride, void* d_dL_dinput, uint64_t dL_dinput_stride, void* d_dL_dweights,
+                       void* d_dL_dbias, n2_grad_mode mode, void* d_workspace, uint64_t workspace_bytes);
+
+/* y = (x - mean) * rstd * scale + shift for each row, mean and variance (over the row, divided by width) in fp32,
+ * rstd = 1 / sqrt(variance + epsilon).  width is 1 to 16384; epsilon > 0.
+ *  dtype, weights_dtype  the type of the rows; that of d_scale and d_shift ([width] each): the same or F32
+ *  d_mean, d_rstd        NULL or fp32 [n_rows], written: what the backward pass reads */
+int n2_layer_norm_forward(n2_stream_t stream, n2_dtype dtype, n2_dtype weights_dtype, uint32_t n_rows, uint32_t width, float epsilon,
+                          const void* d_scale, const void* d_shift, const void* d_input, uint64_t input_stride, void* d_output,
+                          uint64_t output_stride, float* d_mean, float* d_rstd);
+
+/* With xh = (x - mean) * rstd and h = dL/dy * scale, means over the row:
+ *   dL/dx = rstd * (h - mean(h) - xh * mean(h * xh)) + dL/dskip,  dL/dscale = column sums of dL/dy * xh,  dL/dshift = column sums of dL/dy
+ *  d_dL_dskip   NULL or [n_rows][width]: the gradient that reaches x past the norm (a residual block's skip connection)
+ *  d_dL_dinput  NULL or [n_rows][width], written
+ *  d_dL_dscale, d_dL_dshift  [width] in weights_dtype, as the linear layer's (both or neither)
+ *  d_workspace  n2_layer_norm_workspace_bytes(dtype, n_rows, width) bytes, 16-byte aligned; not read with IGNORE */
+uint64_t n2_layer_norm_workspace_bytes(n2_dtype dtype, uint32_t n_rows, uint32_t width);
+int n2_layer_norm_backward(n2_stream_t stream, n2_dtype dtype, n2_dtype weights_dtype, uint32_t n_rows, uint32_t width, const void* d_scale,
+                           const void* d_input, uint64_t input_stride, const float* d_mean, const float* d_rstd, const void* d_dL_doutput,
+                           uint64_t dL_doutput_stride, const void* d_dL_dskip, uint64_t dL_dskip_stride, void* d_dL_dinput,
+                           uint64_t dL_dinput_stride, void* d_dL_dscale, void* d_dL_dshift, n2_grad_mode mode, void* d_workspace,
+                           uint64_t workspace_bytes);
+
+/* The norm over the gradients of many tensors, and clipping.  An object holds the addresses and sizes of the tensors
+ * (host memory only); their contents are read by every call.
+ *   norm = sqrt(sum of squares of all gradients) / loss_scale, summed in fp64: no square overflows or vanishes
+ *   factor = min(1, max_norm / (norm + 1e-6)); out = gradient * factor (loss_scale stays in them)
+ * A norm that is no number makes every gradient one; an infinite one makes finite gradients zero and infinite ones no
+ * numbers.  In place and with a factor of 1 nothing is written. */
+typedef struct n2_gradients n2_gradients_t;
+typedef struct n2_gradient_tensor {
+	const void* d_gradients; /* n values of dtype, without gaps */
+	void* d_out;             /* where the clipped ones go, same type and size: d_gradients itself, or memory of its own */
+	uint64_t n;
+	uint32_t dtype;          /* n2_dtype */
+} n2_gradient_tensor;
+/* The tensors must not overlap each other.  d_table: n2_gradients_table_bytes of device memory, 16-byte aligned, the
+ * object's until it is destroyed; the call fills it and waits for that on the host (not under stream capture). */
+uint64_t n2_gradients_table_bytes(uint32_t n_tensors, const n2_gradient_tensor* tensors);
+int n2_gradients_create(n2_stream_t stream, uint32_t n_tensors, const n2_gradient_tensor* tensors, void* d_table, uint64_t table_bytes,
+                        n2_gradients_t** out);
+void n2_gradients_destroy(n2_gradients_t* gradients);
+/* d_norm: one float, written.  d_workspace: N2_GRADIENTS_WORKSPACE_BYTES, 16-byte aligned.  max_norm >= 0. */
+#define N2_GRADIENTS_WORKSPACE_BYTES 16384u
+int n2_gradients_norm(const n2_gradients_t* gradients, n2_stream_t stream, float loss_scale, float* d_norm, void* d_workspace, uint64_t workspace_bytes);
+int n2_gradients_clip(const n2_gradients_t* gradients, n2_stream_t stream, float max_norm, float loss_scale, float* d_norm, void* d_workspace,
+                      uint64_t workspace_bytes);
+
+/* ------------------------------------------------------------------------
  * Optional event timing of the dominant kernels (off by default; the reference has only
  * wall-clock timers, src/testbed.cu:2707-2710).  When enabled, every launch of a listed kernel is
  * bracketed by a pair of events on its own stream.

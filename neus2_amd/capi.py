@@ -12,6 +12,9 @@ LIB_PATH = os.path.join(_PKG, "libneus2_amd.so")
 N2_OK = 0
 GRAD_IGNORE, GRAD_OVERWRITE, GRAD_ACCUMULATE = 0, 1, 2
 LAYOUT_SOA, LAYOUT_AOS = 0, 1
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
+ACTIVATION_NONE, ACTIVATION_RELU, ACTIVATION_SILU, ACTIVATION_GELU = 0, 1, 2, 3
+GRADIENTS_WORKSPACE_BYTES = 16384
 
 _lib = None
 
@@ -70,6 +73,11 @@ class OccupancyBuffers(C.Structure):
                 ("ema_step", C.c_uint32), ("n_uniform", C.c_uint32), ("rng_state", C.c_uint64), ("rng_inc", C.c_uint64)]
 
 
+class GradientTensor(C.Structure):
+    """struct n2_gradient_tensor"""
+    _fields_ = [("d_gradients", C.c_void_p), ("d_out", C.c_void_p), ("n", C.c_uint64), ("dtype", C.c_uint32)]
+
+
 class SdfBuffers(C.Structure):
     """struct n2_sdf_buffers"""
     _fields_ = [(name, C.c_void_p) for name in ("input", "dy_dx", "output", "dsdf_dinput", "normal", "dL_doutput", "dL_dnormal", "second_order_input", "dL_dinput",
@@ -83,6 +91,8 @@ _SIGNATURES = {
     "n2_field_forward": "pppup", "n2_field_backward": "pppupui", "n2_field_sdf": "pppuuup", "n2_field_density": "pppuuup",
     "n2_sdf_forward_and_loss": "ppppuuuffp", "n2_sdf_loss_backward": "ppppuuupi",
     "n2_trainer_set_training_step": "pu", "n2_trainer_step": "ppuuu", "n2_occupancy_update": "pppfuu",
+    "n2_linear_forward": "piiuuupppqpqpqpqpq", "n2_linear_backward": "piiuuuppqpqpqpqppipq", "n2_layer_norm_forward": "piiuufpppqpqpp",
+    "n2_layer_norm_backward": "piiuuppqpppqpqpqppipq", "n2_gradients_create": "puppqp", "n2_gradients_norm": "ppfppq", "n2_gradients_clip": "ppffppq",
     "n2_marching_cubes_count": "ppppfppqpp", "n2_marching_cubes_count_totals": "ppppfppqpp", "n2_marching_cubes_emit": "ppppfpppppuu",
 }
 
@@ -149,6 +159,12 @@ def lib():
         L.n2_field_destroy.argtypes = [C.c_void_p]
         L.n2_occupancy_workspace_bytes.restype = C.c_uint64
         L.n2_occupancy_workspace_bytes.argtypes = [C.c_void_p, C.c_uint32, C.c_uint32]
+        for name, arguments in (("n2_linear_forward_workspace_bytes", "uuu"), ("n2_linear_backward_workspace_bytes", "uuu"), ("n2_layer_norm_workspace_bytes", "iuu"),
+                                ("n2_gradients_table_bytes", "up")):
+            getattr(L, name).restype = C.c_uint64
+            getattr(L, name).argtypes = [kinds[k] for k in arguments]
+        L.n2_gradients_destroy.restype = None
+        L.n2_gradients_destroy.argtypes = [C.c_void_p]
         L.n2_snapshot_close.restype = None
         L.n2_snapshot_close.argtypes = [C.c_void_p]
         L.n2_occupancy_destroy.restype = None

@@ -1,0 +1,203 @@
+// The norm over the gradients of many tensors and their clipping: two launches whatever the number of tensors.
+// The host cuts the tensors into pieces of PIECE values; a launch's workgroups take pieces in turn.  What bounds both launches
+// is memory: the first reads every gradient, the second reads and writes it, from the last pieces to the first, so that what the first
+// launch read last is still in the caches.
+#include "layer_types.h"
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+namespace {
+
+struct Piece {
+	const void* in;
+	void* out;
+	uint32_t n, dtype;
+	uint64_t unused;
+};
+static_assert(sizeof(Piece) == 32, "pieces are read by 16 bytes");
+
+constexpr uint32_t THREADS = 256, PIECE = 8192, MAX_BLOCKS = N2_GRADIENTS_WORKSPACE_BYTES / sizeof(double) / 2;
+
+// Squares are summed in fp64: those of fp32 and bf16 leave fp32's range long before the values do.
+// (Those of fp16 are exact in fp32, and eight of them lie well inside its range.)
+template <typename T>
+__device__ __forceinline__ double squares(const N2Vec<T>& v) {
+	double s = 0.;
+#pragma unroll
+	for (uint32_t i = 0; i < N2Vec<T>::SIZE; ++i) s = fma((double)(float)v.v[i], (double)(float)v.v[i], s);
+	return s;
+}
+template <>
+__device__ __forceinline__ double squares<n2_f16>(const N2Vec<n2_f16>& v) {
+	float s = 0.f;
+#pragma unroll
+	for (uint32_t i = 0; i < 8u; ++i) s = fmaf((float)v.v[i], (float)v.v[i], s);
+	return (double)s;
+}
+
+template <typename T>
+__device__ __forceinline__ double piece_squares(const Piece& p) {
+	constexpr uint32_t VEC = N2Vec<T>::SIZE;
+	double s = 0.;
+#pragma unroll 4
+	for (uint32_t at = threadIdx.x * VEC; at < p.n; at += THREADS * VEC) s += squares(n2_load_vec(static_cast<const T*>(p.in) + at, n2_left<T>(p.n, at)));
+	return s;
+}
+
+template <typename T>
+__device__ __forceinline__ void piece_scale(const Piece& p, float factor) {
+	constexpr uint32_t VEC = N2Vec<T>::SIZE;
+#pragma unroll 4
+	for (uint32_t at = threadIdx.x * VEC; at < p.n; at += THREADS * VEC) {
+		const uint32_t n = n2_left<T>(p.n, at);
+		N2Vec<T> v = n2_load_vec(static_cast<const T*>(p.in) + at, n);
+#pragma unroll
+		for (uint32_t i = 0; i < VEC; ++i) v.v[i] = (T)((float)v.v[i] * factor);
+		n2_store_vec(static_cast<T*>(p.out) + at, v, n);
+	}
+}
+
+// sum over the workgroup, in all of its lanes
+__device__ __forceinline__ double block_sum(double s) {
+	__shared__ double part[THREADS / 64];
+#pragma unroll
+	for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+	__syncthreads();
+	if ((threadIdx.x & 63u) == 0u) part[threadIdx.x >> 6] = s;
+	__syncthreads();
+	return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__global__ void __launch_bounds__(THREADS) gradient_squares_kernel(const Piece* __restrict__ pieces, uint32_t n_pieces, double* __restrict__ partial) {
+	double s = 0.;
+	for (uint32_t i = blockIdx.x; i < n_pieces; i += gridDim.x) {
+		const Piece p = pieces[i];
+		s += p.dtype == N2_DTYPE_F16 ? piece_squares<n2_f16>(p) : p.dtype == N2_DTYPE_BF16 ? piece_squares<n2_bf16>(p) : piece_squares<float>(p);
+	}
+	s = block_sum(s);
+	if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+__device__ __forceinline__ double norm_of(const double* __restrict__ partial, uint32_t n_partial, double loss_scale) {
+	double s = 0.;
+	for (uint32_t i = threadIdx.x; i < n_partial; i += THREADS) s += partial[i];
+	return sqrt(block_sum(s)) / loss_scale;
+}
+
+__global__ void __launch_bounds__(THREADS) gradient_norm_kernel(const double* __restrict__ partial, uint32_t n_partial, float loss_scale, float* __restrict__ norm) {
+	const double n = norm_of(partial, n_partial, (double)loss_scale);
+	if (threadIdx.x == 0) *norm = (float)n;
+}
+
+// Every workgroup forms the norm itself, from the same sums in the same order.
+__global__ void __launch_bounds__(THREADS) gradient_clip_kernel(const Piece* __restrict__ pieces, uint32_t n_pieces, const double* __restrict__ partial, uint32_t n_partial, float max_norm,
+                                                                float loss_scale, float* __restrict__ norm) {
+	const double n = norm_of(partial, n_partial, (double)loss_scale), ratio = (double)max_norm / (n + 1e-6);
+	const float factor = ratio > 1. ? 1.f : (float)ratio;  // (no number stays none)
+	if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+	for (uint32_t i = blockIdx.x; i < n_pieces; i += gridDim.x) {
+		const Piece p = pieces[n_pieces - 1u - i];
+		if (p.in == p.out && factor == 1.f) continue;
+		if (p.dtype == N2_DTYPE_F16) piece_scale<n2_f16>(p, factor);
+		else if (p.dtype == N2_DTYPE_BF16) piece_scale<n2_bf16>(p, factor);
+		else piece_scale<float>(p, factor);
+	}
+}
+
+uint64_t pieces_of(uint64_t n) { return n / PIECE + (n % PIECE != 0); }
+
+}  // namespace
+
+struct n2_gradients {
+	const Piece* table = nullptr;
+	uint32_t n_pieces = 0, blocks = 0;
+};
+
+N2_API uint64_t n2_gradients_table_bytes(uint32_t n_tensors, const n2_gradient_tensor* tensors) {
+	if (n_tensors > 0 && tensors == nullptr) return 0;
+	uint64_t pieces = 0;
+	for (uint32_t i = 0; i < n_tensors; ++i) pieces += pieces_of(tensors[i].n);
+	return std::max<uint64_t>(pieces, 1) * sizeof(Piece);
+}
+
+N2_API int n2_gradients_create(n2_stream_t stream, uint32_t n_tensors, const n2_gradient_tensor* tensors, void* d_table, uint64_t table_bytes, n2_gradients_t** out) {
+	N2_REQUIRE(out != nullptr, "n2_gradients_create: out is null");
+	*out = nullptr;
+	N2_REQUIRE(n_tensors == 0 || tensors != nullptr, "n2_gradients_create: null tensors");
+	try {
+		struct Range { uintptr_t begin, end; };
+		std::vector<Range> ranges;
+		std::vector<Piece> pieces;
+		for (uint32_t i = 0; i < n_tensors; ++i) {
+			const n2_gradient_tensor& t = tensors[i];
+			N2_REQUIRE(t.dtype <= N2_DTYPE_F32, "n2_gradients_create: tensor %u has type %u", i, t.dtype);
+			if (t.n == 0) continue;
+			const uint64_t bytes = n2_dtype_bytes(t.dtype);
+			N2_REQUIRE(t.d_gradients && t.d_out, "n2_gradients_create: tensor %u is null", i);
+			N2_REQUIRE(t.n < (1ull << 44), "n2_gradients_create: tensor %u has %llu values", i, (unsigned long long)t.n);
+			N2_REQUIRE((reinterpret_cast<uintptr_t>(t.d_gradients) | reinterpret_cast<uintptr_t>(t.d_out)) % bytes == 0, "n2_gradients_create: tensor %u is not aligned to its type", i);
+			const uintptr_t in = reinterpret_cast<uintptr_t>(t.d_gradients), to = reinterpret_cast<uintptr_t>(t.d_out);
+			ranges.push_back({in, in + t.n * bytes});
+			if (to != in) ranges.push_back({to, to + t.n * bytes});
+			for (uint64_t at = 0; at < t.n; at += PIECE)
+				pieces.push_back({static_cast<const char*>(t.d_gradients) + at * bytes, static_cast<char*>(t.d_out) + at * bytes, (uint32_t)std::min<uint64_t>(PIECE, t.n - at), t.dtype, 0});
+		}
+		std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+		for (size_t i = 1; i < ranges.size(); ++i) N2_REQUIRE(ranges[i].begin >= ranges[i - 1].end, "n2_gradients_create: two of the tensors overlap");
+		const uint64_t needed = std::max<uint64_t>(pieces.size(), 1) * sizeof(Piece);
+		N2_REQUIRE(pieces.size() < (1ull << 31), "n2_gradients_create: too many values");
+		N2_REQUIRE(d_table && reinterpret_cast<uintptr_t>(d_table) % 16 == 0 && table_bytes >= needed, "n2_gradients_create: needs a 16-byte aligned table of %llu bytes, got %llu",
+		           (unsigned long long)needed, (unsigned long long)table_bytes);
+		n2_gradients* g = new n2_gradients();
+		g->table = static_cast<const Piece*>(d_table);
+		g->n_pieces = (uint32_t)pieces.size();
+		g->blocks = std::min<uint32_t>(g->n_pieces, MAX_BLOCKS);
+		if (!pieces.empty()) {
+			hipError_t e = hipMemcpyAsync(d_table, pieces.data(), needed, hipMemcpyHostToDevice, n2_stream(stream));
+			if (e == hipSuccess) e = hipStreamSynchronize(n2_stream(stream));
+			if (e != hipSuccess) {
+				delete g;
+				n2_set_error("n2_gradients_create: %s", hipGetErrorString(e));
+				return N2_ERR_HIP;
+			}
+		}
+		*out = g;
+		return N2_OK;
+	} catch (const std::bad_alloc&) {
+		n2_set_error("n2_gradients_create: out of host memory");
+		return N2_ERR_INVALID_ARGUMENT;
+	}
+}
+
+N2_API void n2_gradients_destroy(n2_gradients_t* gradients) { delete gradients; }
+
+static int launch_squares(const n2_gradients_t* g, n2_stream_t stream, float loss_scale, float* d_norm, void* d_workspace, uint64_t workspace_bytes, const char* name) {
+	N2_REQUIRE(g != nullptr && d_norm != nullptr, "%s: null argument", name);
+	N2_REQUIRE(std::isfinite(loss_scale) && loss_scale > 0.f, "%s: loss_scale must be positive", name);
+	N2_REQUIRE(d_workspace && reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0 && workspace_bytes >= N2_GRADIENTS_WORKSPACE_BYTES, "%s: needs a 16-byte aligned workspace of %u bytes, got %llu",
+	           name, N2_GRADIENTS_WORKSPACE_BYTES, (unsigned long long)workspace_bytes);
+	if (g->blocks > 0) {
+		gradient_squares_kernel<<<dim3(g->blocks), dim3(THREADS), 0, n2_stream(stream)>>>(g->table, g->n_pieces, static_cast<double*>(d_workspace));
+		N2_LAUNCH_CHECK();
+	}
+	return N2_OK;
+}
+
+N2_API int n2_gradients_norm(const n2_gradients_t* gradients, n2_stream_t stream, float loss_scale, float* d_norm, void* d_workspace, uint64_t workspace_bytes) {
+	if (const int rc = launch_squares(gradients, stream, loss_scale, d_norm, d_workspace, workspace_bytes, "n2_gradients_norm")) return rc;
+	gradient_norm_kernel<<<dim3(1), dim3(THREADS), 0, n2_stream(stream)>>>(static_cast<const double*>(d_workspace), gradients->blocks, loss_scale, d_norm);
+	N2_LAUNCH_CHECK();
+	return N2_OK;
+}
+
+N2_API int n2_gradients_clip(const n2_gradients_t* gradients, n2_stream_t stream, float max_norm, float loss_scale, float* d_norm, void* d_workspace, uint64_t workspace_bytes) {
+	N2_REQUIRE(max_norm >= 0.f, "n2_gradients_clip: max_norm %g must not be negative", (double)max_norm);
+	if (const int rc = launch_squares(gradients, stream, loss_scale, d_norm, d_workspace, workspace_bytes, "n2_gradients_clip")) return rc;
+	gradient_clip_kernel<<<dim3(std::max(gradients->blocks, 1u)), dim3(THREADS), 0, n2_stream(stream)>>>(gradients->table, gradients->n_pieces, static_cast<const double*>(d_workspace),
+		gradients->blocks, max_norm, loss_scale, d_norm);
+	N2_LAUNCH_CHECK();
+	return N2_OK;
+}

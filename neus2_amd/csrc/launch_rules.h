@@ -269,3 +269,31 @@ static inline N2GatherGrid n2_rows_of_blocks(uint32_t blocks, uint32_t threads) 
 	const uint32_t y = blocks / most + (blocks % most != 0u), x = blocks / y + (blocks % y != 0u);
 	return {(x + N2_XCDS - 1u) / N2_XCDS * N2_XCDS, y};
 }
+
+// Workgroups of a layer norm's launch, each taking groups of rows as far apart as there are workgroups.
+static inline uint32_t n2_layer_norm_blocks(uint32_t n_rows, uint32_t rows_per_block, uint32_t threads) {
+	const uint32_t needed = n_rows / rows_per_block + (n_rows % rows_per_block != 0u), most = threads > 256u ? 512u : 1024u;
+	return needed < most ? needed : most;
+}
+
+static inline uint32_t n2_ceil_div(uint64_t n, uint32_t by) { return (uint32_t)((n + by - 1u) / by); }
+
+// Workgroups along the rows of a linear layer's pass over dz, each leaving a row of column sums.
+static inline uint32_t n2_linear_sum_blocks(uint32_t n_rows, uint32_t out_width) {
+	const uint32_t columns = n2_ceil_div(out_width, 512u), most = 1024u / columns > 16u ? 1024u / columns : 16u, needed = n2_ceil_div(n_rows, 4u);
+	return needed < most ? needed : most;
+}
+
+// The weights' gradient of a linear layer is a product over all rows: where its tiles are fewer than the CUs, the rows are dealt out to
+// several workgroups for each tile, which leave fp32 sums.
+struct N2LinearSplit {
+	uint32_t splits, rows;
+};
+static inline N2LinearSplit n2_linear_gradient_split(uint32_t n_rows, uint32_t in_width, uint32_t out_width) {
+	const uint64_t tiles = (uint64_t)n2_ceil_div(in_width, 128u) * n2_ceil_div(out_width, 128u);
+	const uint64_t most = n2_ceil_div(n_rows, 256u), wanted = 512u / tiles;
+	const uint64_t splits = wanted < most ? wanted : most;
+	if (splits <= 1) return {1, n_rows};
+	const uint32_t rows = n2_ceil_div(n2_ceil_div(n_rows, (uint32_t)splits), 64u) * 64u;
+	return {n2_ceil_div(n_rows, rows), rows};
+}

@@ -1,0 +1,415 @@
+// Linear layers of any width: y = act(x W^T + b) + r, and the two products of the backward pass, dx = dz W and dW = dz^T x.
+// One kernel serves the three products, C[m][n] = sum_k A(m, k) B(n, k), with each operand either contiguous in k (rows of x, W, dz as they
+// stand) or in its own index (W in dx, dz and x in dW): such a tile goes into LDS as it stands in memory and is turned around on the way
+// into the registers (ds_read_b64_tr_b16), so nothing is transposed in memory.
+#include "column_sums.h"
+
+#include <type_traits>
+
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x4 mfma(n2_f16, s16x8 a, s16x8 b, f32x4 c) {
+	return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(n2_bf16, s16x8 a, s16x8 b, f32x4 c) {
+	return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float activation(float z, int kind) {
+	if (kind == N2_ACTIVATION_RELU) return z > 0.f ? z : 0.f;
+	if (kind == N2_ACTIVATION_SILU) return z / (1.f + expf(-z));
+	if (kind == N2_ACTIVATION_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+	return z;
+}
+__device__ __forceinline__ float activation_slope(float z, int kind) {
+	if (kind == N2_ACTIVATION_RELU) return z > 0.f ? 1.f : 0.f;
+	if (kind == N2_ACTIVATION_SILU) {
+		const float s = 1.f / (1.f + expf(-z));
+		return s * (1.f + z * (1.f - s));
+	}
+	if (kind == N2_ACTIVATION_GELU) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+	return 1.f;
+}
+
+// -------------------------------------------------------------------------------------------------------------------------------------
+// tiles
+// -------------------------------------------------------------------------------------------------------------------------------------
+constexpr uint32_t BK = 64;
+
+struct Operand {
+	const void* p;
+	uint64_t ld;
+};
+
+// A tile of R indices by BK in LDS, 16 bytes (eight values) at a time.  Contiguous in k: R rows of eight pieces.  Contiguous in its own
+// index: BK rows of R / 8 pieces.  Pieces of a row are permuted so that the lanes that read one column of pieces meet different banks.
+template <bool KC, uint32_t R, uint32_t RUN>
+__device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
+	if constexpr (KC) {
+		// the 16 rows of a fragment: consecutive ones, or four runs of four that stand RUN apart
+		const uint32_t f = RUN == 4u ? row % 8u : row % 4u + row / RUN % 2u * 4u;
+		return row * (BK / 8u) + (piece ^ f);
+	} else {
+		// a half wave reads 32 bytes of each of the rows k .. k + 3 and k + 8 .. k + 11
+		const uint32_t f = 2u * (row % 4u) + (R >= 128u ? row / 8u % 2u * 8u : 0u);
+		return row * (R / 8u) + (piece ^ f);
+	}
+}
+
+// the tile from index `first` and k0 on; what lies past the extent or past K is zero
+template <typename T, bool KC, uint32_t R, uint32_t RUN, uint32_t THREADS>
+__device__ __forceinline__ void load_tile(uint4* __restrict__ lds, const Operand& o, uint32_t first, uint32_t extent, uint32_t k0, uint32_t k_end) {
+	const T* __restrict__ p = static_cast<const T*>(o.p);
+	constexpr uint32_t PIECES = R * BK / 8u, ROW = KC ? BK / 8u : R / 8u;
+#pragma unroll
+	for (uint32_t i = 0; i < PIECES / THREADS; ++i) {
+		const uint32_t at = i * THREADS + threadIdx.x, row = at / ROW, piece = at % ROW;
+		uint32_t valid;
+		uint64_t from;
+		if constexpr (KC) {
+			valid = first + row < extent && k0 + piece * 8u < k_end ? min(k_end - (k0 + piece * 8u), 8u) : 0u;
+			from = (uint64_t)(first + row) * o.ld + k0 + piece * 8u;
+		} else {
+			valid = k0 + row < k_end && first + piece * 8u < extent ? min(extent - (first + piece * 8u), 8u) : 0u;
+			from = (uint64_t)(k0 + row) * o.ld + first + piece * 8u;
+		}
+		lds[place<KC, R, RUN>(row, piece)] = __builtin_bit_cast(uint4, n2_load_vec(p + from, valid));
+	}
+}
+
+// One operand of a matrix instruction: 16 indices by 32 values of k, lane l holding index l % 16 and the eight values from 8 * (l / 16) on.
+// The 16 indices are base + (i / 4) * RUN + i % 4.
+template <bool KC, uint32_t R, uint32_t RUN>
+__device__ __forceinline__ s16x8 fragment(const uint4* lds, uint32_t base, uint32_t kk) {
+	const uint32_t lane = threadIdx.x & 63u, i = lane % 16u, g = lane / 16u;
+	if constexpr (KC) {
+		return __builtin_bit_cast(s16x8, lds[place<KC, R, RUN>(base + i / 4u * RUN + i % 4u, kk * 4u + g)]);
+	} else {
+		static_assert(RUN == 4u, "");
+		typedef __attribute__((address_space(3))) s16x4* Half;
+		s16x8 r;
+#pragma unroll
+		for (uint32_t h = 0; h < 2u; ++h) {
+			const uint32_t k = kk * 32u + g * 8u + h * 4u + i / 4u, m = base + i % 4u * 4u;
+			const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Half)(reinterpret_cast<const s16x4*>(lds + place<KC, R, RUN>(k, m / 8u)) + m / 4u % 2u));
+			r[h * 4 + 0] = v[0], r[h * 4 + 1] = v[1], r[h * 4 + 2] = v[2], r[h * 4 + 3] = v[3];
+		}
+		return r;
+	}
+}
+
+// -------------------------------------------------------------------------------------------------------------------------------------
+// the product
+// -------------------------------------------------------------------------------------------------------------------------------------
+enum Epilogue { LAYER, STORE, GRADIENT, PARTIAL };
+
+struct Product {
+	Operand a, b;
+	uint32_t m, n, k;
+	uint32_t tiles_m, tiles_n, k_per_split;
+	void* c;              // T [m][n], PARTIAL: fp32 [splits][m][n]
+	uint64_t ldc;
+	// LAYER
+	const void* bias;
+	const void* residual;
+	uint64_t ldr;
+	void* pre;
+	uint64_t ldp;
+	int activation;
+	int accumulate;  // GRADIENT
+};
+
+template <typename T, uint32_t N>
+__device__ __forceinline__ void store_run(T* p, const float (&v)[N], uint32_t valid) {
+	T t[N];
+#pragma unroll
+	for (uint32_t i = 0; i < N; ++i) t[i] = (T)v[i];
+	if (valid >= N) {
+		__builtin_memcpy(p, t, sizeof(t));
+	} else {
+#pragma unroll
+		for (uint32_t i = 0; i < N; ++i)
+			if (i < valid) p[i] = t[i];
+	}
+}
+template <typename T, uint32_t N>
+__device__ __forceinline__ void add_run(float (&v)[N], const T* p, uint32_t valid) {
+	T t[N];
+	if (valid >= N) {
+		__builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+		for (uint32_t i = 0; i < N; ++i) v[i] += (float)t[i];
+	} else {
+#pragma unroll
+		for (uint32_t i = 0; i < N; ++i)
+			if (i < valid) v[i] += (float)p[i];
+	}
+}
+
+// N consecutive values of row m from column n on
+template <typename T, int EPI, uint32_t N>
+__device__ __forceinline__ void finish(const Product& q, uint32_t m, uint32_t n, uint32_t split, float (&v)[N]) {
+	if (m >= q.m || n >= q.n) return;
+	const uint32_t valid = min(q.n - n, N);
+	if constexpr (EPI == PARTIAL) {
+		store_run(static_cast<float*>(q.c) + ((uint64_t)split * q.m + m) * q.n + n, v, valid);
+	} else {
+		T* c = static_cast<T*>(q.c) + (uint64_t)m * q.ldc + n;
+		if constexpr (EPI == LAYER) {
+			if (q.bias != nullptr) add_run(v, static_cast<const T*>(q.bias) + n, valid);
+			if (q.pre != nullptr) store_run(static_cast<T*>(q.pre) + (uint64_t)m * q.ldp + n, v, valid);
+#pragma unroll
+			for (uint32_t i = 0; i < N; ++i) v[i] = activation(v[i], q.activation);
+			if (q.residual != nullptr) add_run(v, static_cast<const T*>(q.residual) + (uint64_t)m * q.ldr + n, valid);
+		}
+		if constexpr (EPI == GRADIENT)
+			if (q.accumulate) add_run(v, c, valid);
+		store_run(c, v, valid);
+	}
+}
+
+// BM x BN of C to a workgroup, WM x WN waves.  The matrix instruction's rows are n and its columns m, so that a lane's four values stand side
+// by side in a row of C; where B is contiguous in k its rows are dealt to the instructions so that all of a lane's values do.
+template <typename T, bool A_KC, bool B_KC, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, int EPI>
+__global__ void __launch_bounds__(WM* WN * 64) product_kernel(Product q) {
+	constexpr uint32_t THREADS = WM * WN * 64u, S = BM / WM / 16u, U = BN / WN / 16u, RUN = B_KC ? 4u * U : 4u;
+	__shared__ uint4 tile_a[BM * BK / 8u], tile_b[BN * BK / 8u];
+	const uint32_t tile = blockIdx.x % (q.tiles_m * q.tiles_n), split = blockIdx.x / (q.tiles_m * q.tiles_n);
+	const uint32_t m0 = tile / q.tiles_n * BM, n0 = tile % q.tiles_n * BN;
+	const uint32_t wave = threadIdx.x / 64u, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+	const uint32_t k_begin = split * q.k_per_split, k_end = min(q.k, k_begin + q.k_per_split);
+	f32x4 acc[S][U] = {};
+	for (uint32_t k0 = k_begin; k0 < k_end; k0 += BK) {
+		load_tile<T, A_KC, BM, 4u, THREADS>(tile_a, q.a, m0, q.m, k0, k_end);
+		load_tile<T, B_KC, BN, RUN, THREADS>(tile_b, q.b, n0, q.n, k0, k_end);
+		__syncthreads();
+#pragma unroll
+		for (uint32_t kk = 0; kk < BK / 32u; ++kk) {
+			s16x8 a[S], b[U];
+#pragma unroll
+			for (uint32_t s = 0; s < S; ++s) a[s] = fragment<A_KC, BM, 4u>(tile_a, wm + s * 16u, kk);
+#pragma unroll
+			for (uint32_t u = 0; u < U; ++u) b[u] = fragment<B_KC, BN, RUN>(tile_b, wn + u * (B_KC ? 4u : 16u), kk);
+#pragma unroll
+			for (uint32_t s = 0; s < S; ++s)
+#pragma unroll
+				for (uint32_t u = 0; u < U; ++u) acc[s][u] = mfma(T{}, b[u], a[s], acc[s][u]);
+		}
+		__syncthreads();
+	}
+	const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+	for (uint32_t s = 0; s < S; ++s) {
+		const uint32_t m = m0 + wm + s * 16u + lane % 16u;
+		if constexpr (B_KC) {
+			float v[4u * U];
+#pragma unroll
+			for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+				for (uint32_t r = 0; r < 4u; ++r) v[u * 4u + r] = acc[s][u][r];
+			finish<T, EPI>(q, m, n0 + wn + lane / 16u * RUN, split, v);
+		} else {
+#pragma unroll
+			for (uint32_t u = 0; u < U; ++u) {
+				float v[4] = {acc[s][u][0], acc[s][u][1], acc[s][u][2], acc[s][u][3]};
+				finish<T, EPI>(q, m, n0 + wn + u * 16u + lane / 16u * 4u, split, v);
+			}
+		}
+	}
+}
+
+// -------------------------------------------------------------------------------------------------------------------------------------
+// dz = dy * act'(z), and its column sums
+// -------------------------------------------------------------------------------------------------------------------------------------
+// A workgroup takes 64 * VEC columns and rows gridDim.y * 4 apart, a wave a row at a time.  dz (or null) goes into rows of ld_dz values, a
+// multiple of eight, zero behind the width; partial (or null): one row of sums from each workgroup.
+template <typename T>
+__global__ void __launch_bounds__(256) slope_kernel(uint32_t n_rows, uint32_t width, const T* __restrict__ dy, uint64_t ld_dy, const T* __restrict__ z, uint64_t ld_z, int kind,
+                                                    T* __restrict__ dz, uint64_t ld_dz, float* __restrict__ partial) {
+	constexpr uint32_t VEC = N2Vec<T>::SIZE;
+	const uint32_t column = (blockIdx.x * 64u + threadIdx.x % 64u) * VEC, wave = threadIdx.x / 64u;
+	const uint32_t n = n2_left<T>(width, column);
+	float sum[VEC] = {};
+	if (column < width) {
+		for (uint64_t row = blockIdx.y * 4u + wave; row < n_rows; row += gridDim.y * 4u) {
+			const N2Vec<T> g = n2_load_vec(dy + row * ld_dy + column, n);
+			N2Vec<T> out = {}, pre = {};
+			if (kind != N2_ACTIVATION_NONE) pre = n2_load_vec(z + row * ld_z + column, n);
+#pragma unroll
+			for (uint32_t i = 0; i < VEC; ++i) {
+				float v = (float)g.v[i];
+				if (kind == N2_ACTIVATION_RELU) v = (float)pre.v[i] > 0.f ? v : 0.f;
+				else if (kind != N2_ACTIVATION_NONE) v *= activation_slope((float)pre.v[i], kind);
+				v = i < n ? v : 0.f;
+				sum[i] += v;
+				out.v[i] = (T)v;
+			}
+			if (dz != nullptr) n2_store_vec(dz + row * ld_dz + column, out, VEC);
+		}
+	}
+	if (partial == nullptr) return;
+	__shared__ float fold[4][64 * VEC];
+#pragma unroll
+	for (uint32_t i = 0; i < VEC; ++i) fold[wave][threadIdx.x % 64u * VEC + i] = sum[i];
+	__syncthreads();
+	for (uint32_t i = threadIdx.x; i < 64u * VEC; i += 256u) {
+		const uint32_t at = blockIdx.x * 64u * VEC + i;
+		if (at < width) partial[(uint64_t)blockIdx.y * width + at] = (fold[0][i] + fold[1][i]) + (fold[2][i] + fold[3][i]);
+	}
+}
+
+template <typename T, bool A_KC, bool B_KC, int EPI>
+int launch_product(hipStream_t s, Product q, uint32_t splits, uint32_t k_per_split) {
+	constexpr uint32_t BM = 128, BN = 128;
+	q.tiles_m = n2_ceil_div(q.m, BM), q.tiles_n = n2_ceil_div(q.n, BN), q.k_per_split = k_per_split;
+	const uint64_t blocks = (uint64_t)q.tiles_m * q.tiles_n * splits;
+	N2_REQUIRE(blocks <= 0xFFFFFFFFull / 256u, "n2_linear: %u x %u values take %llu workgroups", q.m, q.n, (unsigned long long)blocks);
+	product_kernel<T, A_KC, B_KC, BM, BN, 2, 2, EPI><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(q);
+	N2_LAUNCH_CHECK();
+	return N2_OK;
+}
+
+template <typename F>
+int with_type(n2_dtype dtype, F&& f) {
+	return dtype == N2_DTYPE_F16 ? f(n2_f16{}) : f(n2_bf16{});
+}
+
+constexpr uint32_t MAX_WIDTH = 65536;
+
+// what a backward pass keeps in its workspace, in this order
+struct BackwardPlan {
+	uint64_t ld_dz, dz_bytes, sums_bytes, partial_bytes;
+	uint32_t sum_blocks, splits, k_per_split;
+};
+BackwardPlan backward_plan(uint32_t n_rows, uint32_t in_width, uint32_t out_width) {
+	BackwardPlan p = {};
+	p.ld_dz = (uint64_t)n2_ceil_div(out_width, 8u) * 8u;
+	p.dz_bytes = (n_rows * p.ld_dz * 2u + 15u) / 16u * 16u;
+	p.sum_blocks = n2_linear_sum_blocks(n_rows, out_width);
+	p.sums_bytes = ((uint64_t)p.sum_blocks * out_width * 4u + 15u) / 16u * 16u;
+	const N2LinearSplit split = n2_linear_gradient_split(n_rows, in_width, out_width);
+	p.splits = split.splits, p.k_per_split = split.rows;
+	p.partial_bytes = p.splits > 1 ? (uint64_t)p.splits * in_width * out_width * 4u : 0u;
+	return p;
+}
+
+}  // namespace
+
+#define LINEAR_CHECKS(name)                                                                                                                                \
+	N2_REQUIRE(dtype == N2_DTYPE_F16 || dtype == N2_DTYPE_BF16, name ": type %d is neither fp16 nor bf16", (int)dtype);                                    \
+	N2_REQUIRE((int)activation >= N2_ACTIVATION_NONE && (int)activation <= N2_ACTIVATION_GELU, name ": activation %d", (int)activation);                   \
+	N2_REQUIRE(in_width >= 1 && in_width <= MAX_WIDTH && out_width >= 1 && out_width <= MAX_WIDTH, name ": widths %u, %u outside [1, %u]", in_width, out_width, MAX_WIDTH)
+#define STRIDE_CHECK(name, what, pointer, stride, width) \
+	N2_REQUIRE((pointer) == nullptr || n_rows <= 1 || ((stride) >= (width) && n2_rows_fit(n_rows, stride)), name ": the stride of " what " is below the width %u or beyond memory", width)
+
+N2_API uint64_t n2_linear_forward_workspace_bytes(uint32_t n_rows, uint32_t in_width, uint32_t out_width) { return 0; }
+
+N2_API int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation activation, uint32_t n_rows, uint32_t in_width, uint32_t out_width, const void* d_weights,
+                             const void* d_bias, const void* d_input, uint64_t input_stride, const void* d_residual, uint64_t residual_stride, void* d_output, uint64_t output_stride,
+                             void* d_pre_activation, uint64_t pre_stride, void* d_workspace, uint64_t workspace_bytes) {
+	LINEAR_CHECKS("n2_linear_forward");
+	if (n_rows == 0) return N2_OK;
+	N2_REQUIRE(d_weights && d_input && d_output, "n2_linear_forward: null buffer");
+	STRIDE_CHECK("n2_linear_forward", "the input", d_input, input_stride, in_width);
+	STRIDE_CHECK("n2_linear_forward", "the residual", d_residual, residual_stride, out_width);
+	STRIDE_CHECK("n2_linear_forward", "the output", d_output, output_stride, out_width);
+	STRIDE_CHECK("n2_linear_forward", "the saved values", d_pre_activation, pre_stride, out_width);
+	const uint64_t needed = n2_linear_forward_workspace_bytes(n_rows, in_width, out_width);
+	N2_REQUIRE(needed == 0 || (d_workspace && reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0 && workspace_bytes >= needed),
+	           "n2_linear_forward: needs a 16-byte aligned workspace of %llu bytes, got %llu", (unsigned long long)needed, (unsigned long long)workspace_bytes);
+	const bool in_place = d_residual == d_output && (n_rows == 1 || residual_stride == output_stride);
+	const N2Rows written[3] = {n2_rows(d_output, n_rows, out_width, output_stride, 2), n2_rows(d_pre_activation, n_rows, out_width, pre_stride, 2), n2_vector(needed ? d_workspace : nullptr, needed, 1)};
+	const N2Rows read[4] = {n2_vector(d_weights, (uint64_t)in_width * out_width, 2), n2_vector(d_bias, out_width, 2), n2_rows(d_input, n_rows, in_width, input_stride, 2),
+	                        n2_rows(in_place ? nullptr : d_residual, n_rows, out_width, residual_stride, 2)};
+	N2_REQUIRE(!n2_overlap(written, read), "n2_linear_forward: an output overlaps another buffer");
+	Product q = {};
+	q.a = {d_input, input_stride}, q.b = {d_weights, in_width};
+	q.m = n_rows, q.n = out_width, q.k = in_width;
+	q.c = d_output, q.ldc = output_stride;
+	q.bias = d_bias, q.residual = d_residual, q.ldr = residual_stride, q.pre = d_pre_activation, q.ldp = pre_stride, q.activation = activation;
+	return with_type(dtype, [&](auto t) { return launch_product<decltype(t), true, true, LAYER>(n2_stream(stream), q, 1, in_width); });
+}
+
+N2_API uint64_t n2_linear_backward_workspace_bytes(uint32_t n_rows, uint32_t in_width, uint32_t out_width) {
+	if (in_width < 1 || in_width > MAX_WIDTH || out_width < 1 || out_width > MAX_WIDTH) return 0;
+	const BackwardPlan p = backward_plan(n_rows, in_width, out_width);
+	return p.dz_bytes + p.sums_bytes + p.partial_bytes;
+}
+
+N2_API int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation activation, uint32_t n_rows, uint32_t in_width, uint32_t out_width, const void* d_weights,
+                              const void* d_input, uint64_t input_stride, const void* d_pre_activation, uint64_t pre_stride, const void* d_dL_doutput, uint64_t dL_doutput_stride,
+                              void* d_dL_dinput, uint64_t dL_dinput_stride, void* d_dL_dweights, void* d_dL_dbias, n2_grad_mode mode, void* d_workspace, uint64_t workspace_bytes) {
+	LINEAR_CHECKS("n2_linear_backward");
+	N2_REQUIRE(mode == N2_GRAD_IGNORE || mode == N2_GRAD_OVERWRITE || mode == N2_GRAD_ACCUMULATE, "n2_linear_backward: gradient mode %d", (int)mode);
+	void* const dw = mode == N2_GRAD_IGNORE ? nullptr : d_dL_dweights;
+	void* const db = mode == N2_GRAD_IGNORE ? nullptr : d_dL_dbias;
+	if (activation == N2_ACTIVATION_NONE) d_pre_activation = nullptr;
+	if (n_rows > 0) {
+		N2_REQUIRE(d_weights && d_input && d_dL_doutput && (d_pre_activation || activation == N2_ACTIVATION_NONE), "n2_linear_backward: null buffer");
+		STRIDE_CHECK("n2_linear_backward", "the input", d_input, input_stride, in_width);
+		STRIDE_CHECK("n2_linear_backward", "the saved values", d_pre_activation, pre_stride, out_width);
+		STRIDE_CHECK("n2_linear_backward", "the output's gradient", d_dL_doutput, dL_doutput_stride, out_width);
+		STRIDE_CHECK("n2_linear_backward", "the input's gradient", d_dL_dinput, dL_dinput_stride, in_width);
+	}
+	const BackwardPlan p = backward_plan(n_rows, in_width, out_width);
+	const uint64_t needed = p.dz_bytes + p.sums_bytes + p.partial_bytes;
+	N2_REQUIRE(needed == 0 || (d_workspace && reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0 && workspace_bytes >= needed),
+	           "n2_linear_backward: needs a 16-byte aligned workspace of %llu bytes, got %llu", (unsigned long long)needed, (unsigned long long)workspace_bytes);
+	const N2Rows written[4] = {n2_rows(d_dL_dinput, n_rows, in_width, dL_dinput_stride, 2), n2_vector(dw, (uint64_t)in_width * out_width, 2), n2_vector(db, out_width, 2),
+	                           n2_vector(needed ? d_workspace : nullptr, needed, 1)};
+	const N2Rows read[4] = {n2_vector(n_rows ? d_weights : nullptr, (uint64_t)in_width * out_width, 2), n2_rows(d_input, n_rows, in_width, input_stride, 2),
+	                        n2_rows(d_pre_activation, n_rows, out_width, pre_stride, 2), n2_rows(d_dL_doutput, n_rows, out_width, dL_doutput_stride, 2)};
+	N2_REQUIRE(!n2_overlap(written, read), "n2_linear_backward: an output overlaps another buffer");
+	hipStream_t s = n2_stream(stream);
+	const int accumulate = mode == N2_GRAD_ACCUMULATE ? 1 : 0;
+	char* ws = static_cast<char*>(d_workspace);
+	float* const sums = reinterpret_cast<float*>(ws + p.dz_bytes);
+	float* const partial = reinterpret_cast<float*>(ws + p.dz_bytes + p.sums_bytes);
+	return with_type(dtype, [&](auto t) -> int {
+		using T = decltype(t);
+		// dz: the output's gradient itself where there is no activation
+		const bool products = d_dL_dinput != nullptr || dw != nullptr, writes = activation != N2_ACTIVATION_NONE && products;
+		Operand dz = {d_dL_doutput, dL_doutput_stride};
+		if (n_rows > 0 && (writes || db != nullptr)) {
+			if (writes) dz = {ws, p.ld_dz};
+			slope_kernel<T><<<dim3(n2_ceil_div(out_width, 512u), p.sum_blocks), dim3(256), 0, s>>>(n_rows, out_width, static_cast<const T*>(d_dL_doutput), dL_doutput_stride,
+				static_cast<const T*>(d_pre_activation), pre_stride, activation, writes ? reinterpret_cast<T*>(ws) : nullptr, p.ld_dz, db != nullptr ? sums : nullptr);
+			N2_LAUNCH_CHECK();
+		}
+		if (d_dL_dinput != nullptr && n_rows > 0) {
+			Product q = {};
+			q.a = dz, q.b = {d_weights, in_width};
+			q.m = n_rows, q.n = in_width, q.k = out_width;
+			q.c = d_dL_dinput, q.ldc = dL_dinput_stride;
+			if (const int rc = launch_product<T, true, false, STORE>(s, q, 1, out_width)) return rc;
+		}
+		if (dw != nullptr) {
+			Product q = {};
+			q.a = dz, q.b = {d_input, input_stride};
+			q.m = out_width, q.n = in_width, q.k = n_rows;
+			q.c = dw, q.ldc = in_width, q.accumulate = accumulate;
+			if (p.splits <= 1) {
+				if (const int rc = launch_product<T, false, false, GRADIENT>(s, q, 1, n_rows)) return rc;
+			} else {
+				q.c = partial;
+				if (const int rc = launch_product<T, false, false, PARTIAL>(s, q, p.splits, p.k_per_split)) return rc;
+				const uint64_t n = (uint64_t)in_width * out_width;
+				const N2ColumnOutput out = {dw, 0, (uint32_t)n, (uint32_t)dtype};
+				n2_column_sums_kernel<1><<<dim3((uint32_t)((n + N2_SUM_COLUMNS - 1) / N2_SUM_COLUMNS)), dim3(N2_SUM_COLUMNS * N2_SUM_ROWS), 0, s>>>(partial, p.splits, n, (uint32_t)n, out, out, accumulate);
+				N2_LAUNCH_CHECK();
+			}
+		}
+		if (db != nullptr) {
+			const N2ColumnOutput out = {db, 0, out_width, (uint32_t)dtype};
+			n2_column_sums_kernel<1><<<dim3(n2_ceil_div(out_width, N2_SUM_COLUMNS)), dim3(N2_SUM_COLUMNS * N2_SUM_ROWS), 0, s>>>(sums, n_rows > 0 ? p.sum_blocks : 0u, out_width, out_width, out, out, accumulate);
+			N2_LAUNCH_CHECK();
+		}
+		return N2_OK;
+	});
+}

@@ -1,0 +1,524 @@
+"""The layers of any width and the clipping on the GPU, against their formulas in 64 bits (tests/layers_ref.py)."""
+import math
+
+import pytest
+import torch
+
+import layers_ref as ref
+
+pytestmark = pytest.mark.gpu
+HALVES = [torch.float16, torch.bfloat16]
+KINDS = ["None", "ReLU", "SiLU", "GELU"]
+
+
+def _rows(gen, n, w, dtype, extra=0, first=0, scale=1.0):
+    """[n, w] values inside a wider matrix: `extra` columns beside them, starting at element `first`."""
+    whole = (torch.randn(n, w + extra, generator=gen) * scale).to(dtype).cuda() if n else torch.empty(0, w + extra, dtype=dtype, device="cuda")
+    return whole[:, first:first + w]
+
+
+def _canvas(n, w, dtype, extra, first):
+    """An output inside a wider and longer matrix of marks, and the check that only the output was written."""
+    whole = torch.full((n + 3, w + extra), 77.0, dtype=dtype, device="cuda")
+    out = whole[:n, first:first + w]
+
+    def check():
+        rest = whole.clone()
+        rest[:n, first:first + w] = 77.0
+        assert bool((rest == 77.0).all()), "written outside the output"
+    return out, check
+
+
+def _linear(gen, i, o, kind, bias, dtype):
+    from neus2_amd.layers import Linear
+    op = Linear(i, o, activation=kind, bias=bias, dtype=dtype)
+    w = torch.randn(o * i, generator=gen) / math.sqrt(i)
+    params = torch.cat([w, torch.randn(o, generator=gen) * 0.3] if bias else [w]).to(dtype).cuda()
+    op.set_params(params, torch.zeros_like(params))
+    return op, params[:o * i].view(o, i), params[o * i:] if bias else None
+
+
+# rows, in, out, extra columns, first column
+SHAPES = [(1, 1, 1, 0, 0), (1, 256, 256, 0, 0), (2, 3, 5, 3, 1), (16, 512, 96, 8, 8), (17, 200, 33, 0, 0), (64, 64, 64, 0, 0), (65, 63, 129, 1, 1), (128, 128, 128, 0, 0),
+          (130, 257, 31, 0, 0), (300, 72, 257, 8, 0), (513, 320, 257, 7, 3), (1000, 40, 24, 0, 0), (257, 1032, 264, 0, 0), (1500, 16, 8, 0, 0), (700, 500, 300, 4, 4)]
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,i,o,extra,first", SHAPES)
+def test_linear_forward(n, i, o, extra, first, kind, dtype):
+    gen = torch.Generator().manual_seed(n * 31 + i + o)
+    residual = (n + i) % 2 == 0
+    op, w, b = _linear(gen, i, o, kind, bias=o % 3 != 0, dtype=dtype)
+    x = _rows(gen, n, i, dtype, extra, first)
+    r = _rows(gen, n, o, dtype, extra, first) if residual else None
+    out, check = _canvas(n, o, dtype, extra, first)
+    y, z = op.forward(x, residual=r, want_pre_activation=True, out=out)
+    ye, ze, dy, dz = ref.linear_forward(x, w, b, r, kind)
+    ref.within(y, ye, dy, "y")
+    ref.within(z, ze, dz, "z")
+    check()
+    assert torch.equal(op.forward(x, residual=r)[0], y)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,i,o,extra,first", SHAPES)
+def test_linear_backward(n, i, o, extra, first, kind, dtype):
+    from neus2_amd.capi import GRAD_ACCUMULATE, GRAD_IGNORE
+    gen = torch.Generator().manual_seed(n * 17 + i + o)
+    op, w, b = _linear(gen, i, o, kind, bias=True, dtype=dtype)
+    x, dy = _rows(gen, n, i, dtype, extra, first), _rows(gen, n, o, dtype, extra, first)
+    z = _rows(gen, n, o, dtype, extra, first) if kind != "None" else None
+    e = ref.linear_backward(x, w, z, dy, kind)
+    out, check = _canvas(n, i, dtype, extra, first)
+    op._grads.fill_(float("nan"))  # overwritten, whatever stands there
+    op.backward(x, z, dy, out=out)
+    check()
+    grads = op._grads.clone()
+    ref.within(out, *e["dx"], "dx")
+    ref.within(grads[:o * i].view(o, i), *e["dw"], "dw")
+    ref.within(grads[o * i:], *e["db"], "db")
+    # the parts on their own give the same bits
+    op._grads.zero_()
+    assert op.backward(x, z, dy, want_input_grad=False) is None and torch.equal(op._grads, grads)
+    op._grads.fill_(5.0)
+    assert torch.equal(op.backward(x, z, dy, mode=GRAD_IGNORE), out) and bool((op._grads == 5.0).all())
+    # added to what is there, rounded once
+    before = (torch.randn(op.n_params(), generator=gen)).to(dtype).cuda()
+    op._grads.copy_(before)
+    op.backward(x, z, dy, mode=GRAD_ACCUMULATE)
+    old = before.double()
+    ref.within(op._grads[:o * i].view(o, i), e["dw"][0] + old[:o * i].view(o, i), e["dw"][1] + ref.U32 * (e["dw"][0].abs() + old[:o * i].view(o, i).abs()), "dw added")
+    ref.within(op._grads[o * i:], e["db"][0] + old[o * i:], e["db"][1] + ref.U32 * (e["db"][0].abs() + old[o * i:].abs()), "db added")
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("n,i,o", [(20000, 24, 16), (9001, 130, 257), (4096, 256, 256), (2048, 512, 768)])
+def test_linear_backward_sums_many_rows(n, i, o, dtype):
+    """Rows dealt out to several workgroups for each tile of the weights' gradient; twice the same bits."""
+    gen = torch.Generator().manual_seed(n)
+    op, w, b = _linear(gen, i, o, "GELU", bias=True, dtype=dtype)
+    x, z, dy = _rows(gen, n, i, dtype), _rows(gen, n, o, dtype), _rows(gen, n, o, dtype, scale=0.01)
+    dx = op.backward(x, z, dy)
+    grads = op._grads.clone()
+    e = {k: v for k, v in ref.linear_backward(x, w, z, dy, "GELU").items()}
+    ref.within(dx, *e["dx"], "dx")
+    ref.within(grads[:o * i].view(o, i), *e["dw"], "dw")
+    ref.within(grads[o * i:], *e["db"], "db")
+    op._grads.zero_()
+    assert torch.equal(op.backward(x, z, dy), dx) and torch.equal(op._grads, grads)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+def test_linear_of_no_rows(dtype):
+    from neus2_amd.capi import GRAD_ACCUMULATE
+    gen = torch.Generator().manual_seed(1)
+    op, w, b = _linear(gen, 40, 24, "SiLU", bias=True, dtype=dtype)
+    x, g = torch.empty(0, 40, dtype=dtype, device="cuda"), torch.empty(0, 24, dtype=dtype, device="cuda")
+    y, z = op.forward(x, want_pre_activation=True)
+    assert y.shape == z.shape == (0, 24)
+    op._grads.fill_(3.0)
+    op.backward(x, z, g, mode=GRAD_ACCUMULATE)
+    assert bool((op._grads == 3.0).all())
+    assert op.backward(x, z, g).shape == (0, 40) and not bool(op._grads.any())
+
+
+@pytest.mark.parametrize("n", [1, 5, 16, 40, 300])
+def test_infinities_and_nans_stay_in_their_rows(n):
+    """A row of no numbers, beside rows of numbers and behind the last row of the batch, changes no other row."""
+    gen = torch.Generator().manual_seed(n)
+    op, w, b = _linear(gen, 72, 40, "None", bias=True, dtype=torch.float16)
+    whole = _rows(gen, n + 2, 72, torch.float16)
+    clean = op.forward(whole[:n].clone())[0]
+    whole[n:] = float("nan")
+    assert torch.equal(op.forward(whole[:n])[0], clean)
+    if n > 1:
+        whole[n // 2] = float("inf")
+        got = op.forward(whole[:n])[0]
+        others = torch.arange(n) != n // 2
+        assert torch.equal(got[others], clean[others]) and not bool(torch.isfinite(got[n // 2]).any())
+
+
+def test_columns_behind_a_row_are_not_read():
+    """What stands between a row's end and the next row's start may be anything."""
+    gen = torch.Generator().manual_seed(3)
+    for i, o, first in ((72, 40, 0), (65, 33, 1), (8, 8, 8)):
+        op, w, b = _linear(gen, i, o, "ReLU", bias=True, dtype=torch.bfloat16)
+        x, z, dy = (_rows(gen, 90, c, torch.bfloat16) for c in (i, o, o))
+        wide = []
+        for t in (x, z, dy):
+            m = torch.full((90, t.shape[1] + first + 5), float("nan"), dtype=torch.bfloat16, device="cuda")
+            m[:, first:first + t.shape[1]] = t
+            wide.append(m[:, first:first + t.shape[1]])
+        assert torch.equal(op.forward(wide[0])[0], op.forward(x)[0])
+        dx = op.backward(x, z, dy)
+        grads = op._grads.clone()
+        assert torch.equal(op.backward(*wide), dx) and torch.equal(op._grads, grads)
+
+
+def test_residual_in_place_and_columns_of_one_matrix():
+    gen = torch.Generator().manual_seed(4)
+    op, w, b = _linear(gen, 64, 64, "SiLU", bias=True, dtype=torch.float16)
+    x, r = _rows(gen, 200, 64, torch.float16), _rows(gen, 200, 64, torch.float16)
+    y = op.forward(x, residual=r)[0]
+    stream = r.clone()
+    assert op.forward(x, residual=stream, out=stream)[0] is stream and torch.equal(stream, y)
+    both = torch.cat([x, r], 1)  # input and output side by side
+    op.forward(both[:, :64], residual=both[:, 64:], out=both[:, 64:])
+    assert torch.equal(both[:, 64:], y) and torch.equal(both[:, :64], x)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_linear_gradients_against_differences(kind):
+    """<dx, d> against (L(x + h d) - L(x - h d)) / 2h of the forward pass in 64 bits, L = sum(dy * y), and the same for the weights:
+    off by the gradient's own bound along d and the differences' h^2 / 6 times the third derivative (activations: below 2)."""
+    dtype = torch.float16
+    gen = torch.Generator().manual_seed(8)
+    op, w, b = _linear(gen, 24, 20, kind, bias=True, dtype=dtype)
+    x, dy = _rows(gen, 33, 24, dtype), _rows(gen, 33, 20, dtype)
+    z = (x.double() @ w.double().T + b.double())
+    if kind == "ReLU":  # (differences across the corner say nothing)
+        x = x[(z.abs() > 1e-2).all(1)]
+        dy = dy[:x.shape[0]]
+        z = (x.double() @ w.double().T + b.double())
+    zq = z.to(dtype)
+    dx = op.backward(x, zq, dy)
+    dw, db = op._grads[:480].view(20, 24), op._grads[480:]
+    e = ref.linear_backward(x, w, zq, dy, kind)
+    h = 1e-5
+    L = lambda x_, w_, b_: float((dy.double() * ref.act(x_ @ w_.T + b_, kind)).sum())
+    for name, got, at in (("dx", dx, 0), ("dw", dw, 1), ("db", db, 2)):
+        parts = [x.double(), w.double(), b.double()]
+        d = torch.randn(parts[at].shape, generator=gen).double().cuda()
+        up, down = list(parts), list(parts)
+        up[at], down[at] = parts[at] + h * d, parts[at] - h * d
+        numeric = (L(*up) - L(*down)) / (2 * h)
+        bound = e[name][1] + ref.half_step(dtype) * (e[name][0].abs() + e[name][1]) + ref.least(dtype)
+        # (the saved z is rounded: the slope moves by half a step of z times a curvature below 1.2)
+        curvature = 0.0 if kind in ("None", "ReLU") else 1.2
+        moved = curvature * (ref.half_step(dtype) * z.abs()) * dy.double().abs()
+        turned = {"dx": lambda: moved @ w.double().abs(), "dw": lambda: moved.T @ x.double().abs(), "db": lambda: moved.sum(0)}[name]()
+        third = 0.0 if curvature == 0.0 else 2 * h * h / 6 * float((dy.double().abs() * (x.double().abs() @ w.double().abs().T + x.double().abs().sum(1, True) + w.double().abs().sum(1) + 1) ** 3).sum()) * 64
+        assert abs(float((got.double() * d).sum()) - numeric) <= float(((bound + turned) * d.abs()).sum()) + third + 1e-7 * abs(numeric), name
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------------------------------------------------
+TYPES = [(torch.float16, torch.float16), (torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32)]
+NORMS = [(1, 1, 0, 0), (3, 2, 3, 1), (1000, 64, 0, 0), (257, 63, 1, 1), (33, 129, 0, 0), (64, 256, 8, 8), (50, 257, 0, 0), (40, 1000, 8, 0), (21, 1537, 0, 0), (9, 2048, 0, 0), (7, 4097, 3, 2),
+         (5, 8192, 0, 0), (3, 16384, 0, 0), (2100, 24, 0, 0)]
+
+
+def _norm(gen, w, dtype, weights):
+    from neus2_amd.layers import LayerNorm
+    op = LayerNorm(w, dtype=dtype, param_dtype=weights)
+    params = torch.cat([1 + 0.2 * torch.randn(w, generator=gen), 0.3 * torch.randn(w, generator=gen)]).to(weights).cuda()
+    op.set_params(params, torch.zeros_like(params))
+    return op, params[:w], params[w:]
+
+
+@pytest.mark.parametrize("dtype,weights", TYPES)
+@pytest.mark.parametrize("n,w,extra,first", NORMS)
+def test_norm_forward_and_backward(n, w, extra, first, dtype, weights):
+    from neus2_amd.capi import GRAD_ACCUMULATE, GRAD_IGNORE
+    gen = torch.Generator().manual_seed(n + w)
+    op, scale, shift = _norm(gen, w, dtype, weights)
+    x = _rows(gen, n, w, dtype, extra, first)
+    out, check = _canvas(n, w, dtype, extra, first)
+    y, (mean, rstd) = op.forward(x, want_ctx=True, out=out)
+    ye, me, se = ref.norm_forward(x, scale, shift, 1e-5)
+    ref.within(y, *ye, "y")
+    ref.within(mean, *me, "mean")
+    ref.within(rstd, *se, "rstd")
+    check()
+    assert torch.equal(op.forward(x)[0], y)
+    dy, skip = _rows(gen, n, w, dtype, extra, first), _rows(gen, n, w, dtype, extra, first) if w % 2 else None
+    e = ref.norm_backward(x, mean, rstd, scale, dy, skip)
+    dx, check = _canvas(n, w, dtype, extra, first)
+    op._grads.fill_(float("nan"))
+    op.backward((mean, rstd), x, dy, dL_dskip=skip, out=dx)
+    check()
+    grads = op._grads.clone()
+    ref.within(dx, *e["dx"], "dx")
+    ref.within(grads[:w], *e["dscale"], "dscale")
+    ref.within(grads[w:], *e["dshift"], "dshift")
+    assert op.backward((mean, rstd), x, dy, want_input_grad=False) is None and torch.equal(op._grads, grads)
+    op._grads.fill_(2.0)
+    assert torch.equal(op.backward((mean, rstd), x, dy, dL_dskip=skip, mode=GRAD_IGNORE), dx) and bool((op._grads == 2.0).all())
+    op.backward((mean, rstd), x, dy, mode=GRAD_ACCUMULATE)
+    for name, got in (("dscale", op._grads[:w]), ("dshift", op._grads[w:])):
+        ref.within(got, e[name][0] + 2.0, e[name][1] + ref.U32 * (e[name][0].abs() + 2.0), name + " added")
+
+
+def test_norm_of_many_rows():
+    gen = torch.Generator().manual_seed(6)
+    op, scale, shift = _norm(gen, 256, torch.float16, torch.float16)
+    x, dy, skip = (_rows(gen, 30011, 256, torch.float16) for _ in range(3))
+    y, ctx = op.forward(x, want_ctx=True)
+    ref.within(y, *ref.norm_forward(x, scale, shift, 1e-5)[0], "y")
+    dx = op.backward(ctx, x, dy, dL_dskip=skip)
+    e = ref.norm_backward(x, *ctx, scale, dy, skip)
+    ref.within(dx, *e["dx"], "dx")
+    ref.within(op._grads[:256], *e["dscale"], "dscale")
+    ref.within(op._grads[256:], *e["dshift"], "dshift")
+    into = skip.clone()  # the gradient stream in place
+    assert op.backward(ctx, x, dy, dL_dskip=into, out=into) is into and torch.equal(into, dx)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_norm_of_rows_far_from_zero_and_of_equal_values(dtype):
+    """The variance comes of the centred values: a mean a thousand times the deviation takes nothing from it.  Equal values have none."""
+    gen = torch.Generator().manual_seed(7)
+    op, scale, shift = _norm(gen, 96, dtype, torch.float32)
+    x = (torch.randn(20, 96, generator=gen) + 1000).to(dtype).cuda()
+    x[3] = 12.0
+    y, (mean, rstd) = op.forward(x, want_ctx=True)
+    ye, me, se = ref.norm_forward(x, scale, shift, 1e-5)
+    ref.within(y, *ye, "y")
+    ref.within(rstd, *se, "rstd")
+    assert torch.equal(y[3], shift.to(dtype)) and float(rstd[3]) == pytest.approx(1e-5 ** -0.5, rel=1e-6)
+    x[5, 7] = float("inf")
+    x[6, 1] = float("nan")
+    got = op.forward(x)[0]
+    others = torch.tensor([i not in (5, 6) for i in range(20)])
+    assert torch.equal(got[others], y[others]) and bool(got[6].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_norm_of_no_rows(dtype):
+    gen = torch.Generator().manual_seed(9)
+    op, scale, shift = _norm(gen, 48, dtype, dtype)
+    x = torch.empty(0, 48, dtype=dtype, device="cuda")
+    y, ctx = op.forward(x, want_ctx=True)
+    op._grads.fill_(1.0)
+    assert op.backward(ctx, x, y).shape == (0, 48) and not bool(op._grads.any())
+
+
+def test_norm_gradients_against_differences():
+    """Central differences of the forward pass in 64 bits with statistics of its own: h = 1e-5 leaves an error of third derivatives times
+    h^2 (below 1e-7 here) and of cancellation (1e-11 of the sum)."""
+    gen = torch.Generator().manual_seed(10)
+    op, scale, shift = _norm(gen, 40, torch.float32, torch.float32)
+    x, dy, skip = (_rows(gen, 17, 40, torch.float32) for _ in range(3))
+    y, ctx = op.forward(x, want_ctx=True)
+    dx = op.backward(ctx, x, dy, dL_dskip=skip)
+    e = ref.norm_backward(x, *ctx, scale, dy, skip)
+
+    def loss(x_, s_, b_):
+        mean = x_.mean(1, keepdim=True)
+        xh = (x_ - mean) / ((x_ - mean).square().mean(1, keepdim=True) + 1e-5).sqrt()
+        return float((dy.double() * (xh * s_ + b_)).sum() + (skip.double() * x_).sum())
+
+    parts = [x.double(), scale.double(), shift.double()]
+    for at, name, got in ((0, "dx", dx), (1, "dscale", op._grads[:40]), (2, "dshift", op._grads[40:])):
+        d = torch.randn(parts[at].shape, generator=gen).double().cuda()
+        up, down = list(parts), list(parts)
+        up[at], down[at] = parts[at] + 1e-5 * d, parts[at] - 1e-5 * d
+        numeric = (loss(*up) - loss(*down)) / 2e-5
+        # (mean and rstd are the kernel's: relative errors of 50 half steps of fp32)
+        bound = float(((e[name][1] + ref.U32 * e[name][0].abs()) * d.abs()).sum()) + 200 * ref.U32 * float((e[name][0].abs() * d.abs()).sum() + (dy.abs().sum() if at < 2 else 0))
+        assert abs(float((got.double() * d).sum()) - numeric) <= bound + 1e-5, name
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# clipping
+# ---------------------------------------------------------------------------------------------------------------------
+def _gradients(gen, sizes, dtypes, scale=1.0):
+    return [(torch.randn(n, generator=gen) * scale).to(dtypes[i % len(dtypes)]).cuda() for i, n in enumerate(sizes)]
+
+
+ALL = [torch.float16, torch.bfloat16, torch.float32]
+
+
+@pytest.mark.parametrize("sizes", [[1], [7, 0, 8193], [8192] * 3, [100003, 3, 64, 16385, 1], [5] * 700])
+@pytest.mark.parametrize("dtypes", [[t] for t in ALL] + [ALL])
+@pytest.mark.parametrize("apart", [False, True])
+def test_clip(sizes, dtypes, apart):
+    from neus2_amd.layers import GradientClip
+    gen = torch.Generator().manual_seed(sum(sizes))
+    g = _gradients(gen, sizes, dtypes)
+    before = [t.clone() for t in g]
+    norm = math.sqrt(sum(float(t.double().square().sum()) for t in g)) / 128
+    out = [torch.full_like(t, 9.0) for t in g] if apart else None
+    clip = GradientClip(g, out=out)
+    # sums in fp64 (fp16: eight squares at a time in fp32, 8 half steps): the norm rounded once
+    near = pytest.approx(norm, rel=10 * ref.U32)
+    assert float(clip.norm(loss_scale=128.0)) == near
+    assert all(torch.equal(a, b) for a, b in zip(g, before))
+    assert float(clip.clip(2 * norm, loss_scale=128.0)) == near  # below the limit
+    assert all(torch.equal(a, b) for a, b in zip(out if apart else g, before))
+    assert float(clip.clip(0.3 * norm, loss_scale=128.0)) == near
+    factor = 0.3 * norm / (norm + 1e-6)
+    for a, b in zip(out if apart else g, before):
+        ref.within(a, b.double() * factor, 12 * ref.U32 * b.double().abs() * factor, "clipped")
+    if apart:
+        assert all(torch.equal(a, b) for a, b in zip(g, before))
+
+
+def test_clip_reads_what_the_tensors_hold_then():
+    from neus2_amd.layers import GradientClip
+    g = [torch.zeros(5000, device="cuda"), torch.zeros(3, 7, dtype=torch.float16, device="cuda")]
+    clip = GradientClip(g)
+    assert float(clip.norm()) == 0.0 and float(clip.clip(1.0)) == 0.0 and not any(bool(t.any()) for t in g)
+    g[0][17], g[1][2, 3] = 3.0, 4.0
+    assert float(clip.clip(0.5)) == 5.0
+    assert float(g[0][17]) == pytest.approx(0.3, rel=1e-6) and float(g[1][2, 3]) == pytest.approx(0.4, rel=2 ** -11)
+    assert float(GradientClip([]).norm()) == 0.0 and float(GradientClip([]).clip(1.0)) == 0.0
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.float32, 1e30), (torch.float32, 1e-30), (torch.bfloat16, 1e30), (torch.bfloat16, 1e-30), (torch.float16, 6e4), (torch.float16, 6e-8)])
+def test_norm_of_values_whose_squares_leave_fp32(dtype, size):
+    from neus2_amd.layers import GradientClip
+    g = torch.full((4096,), size, device="cuda").to(dtype)
+    exact = 64 * float(g[0])
+    assert float(GradientClip([g]).norm()) == pytest.approx(exact, rel=10 * ref.U32)
+
+
+def test_gradients_that_are_no_numbers():
+    from neus2_amd.layers import GradientClip
+    g = torch.ones(100, device="cuda")
+    g[3] = float("inf")
+    clip = GradientClip([g])
+    assert float(clip.clip(1.0)) == math.inf
+    assert bool(g[3].isnan()) and float(g.nan_to_num(0.0).abs().sum()) == 0.0
+    assert math.isnan(float(clip.clip(1.0))) and bool(g.isnan().all())
+
+
+def test_clipping_is_the_same_every_time():
+    from neus2_amd.layers import GradientClip
+    gen = torch.Generator().manual_seed(2)
+    g = _gradients(gen, [70000, 1 << 20, 333, 12345], ALL)
+    clip = GradientClip(g, out=[torch.empty_like(t) for t in g])
+    runs = [(clip.clip(1.0).clone(), [t.clone() for t in clip._keep[1]]) for _ in range(3)]
+    for norm, out in runs[1:]:
+        assert torch.equal(norm, runs[0][0]) and all(torch.equal(a, b) for a, b in zip(out, runs[0][1]))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------------------------------------------------
+class Block:
+    """x + W2 gelu(W1 norm(x) + b1) + b2, its parameters and gradients in one vector, as the optimiser takes them."""
+
+    def __init__(self, gen, width, hidden):
+        from neus2_amd.layers import LayerNorm, Linear
+        self.ops = [LayerNorm(width), Linear(width, hidden, activation="GELU"), Linear(hidden, width)]
+        sizes = [op.n_params() for op in self.ops]
+        master = [torch.cat([torch.ones(width), torch.zeros(width)])]
+        for i, o in ((width, hidden), (hidden, width)):
+            master.append(torch.cat([torch.randn(o * i, generator=gen) / math.sqrt(i), torch.zeros(o)]))
+        self.master = torch.cat(master).cuda()
+        self.params, self.grads = self.master.half(), torch.zeros(sum(sizes), dtype=torch.float16, device="cuda")
+        self.slices = [slice(sum(sizes[:k]), sum(sizes[:k + 1])) for k in range(3)]
+        for op, s in zip(self.ops, self.slices):
+            op.set_params(self.params[s], self.grads[s])
+
+    def forward(self, x):
+        norm, up, down = self.ops
+        y, ctx = norm.forward(x, want_ctx=True)
+        h, z = up.forward(y, want_pre_activation=True)
+        out, _ = down.forward(h, residual=x)
+        return out, (x, y, ctx, h, z)
+
+    def backward(self, saved, dL_dout):
+        norm, up, down = self.ops
+        x, y, ctx, h, z = saved
+        dh = down.backward(h, None, dL_dout)
+        dy = up.backward(y, z, dh)
+        return norm.backward(ctx, x, dy, dL_dskip=dL_dout), dh, dy
+
+
+@pytest.mark.parametrize("n,width,hidden", [(300, 64, 256), (77, 41, 90)])
+def test_a_training_step_of_a_residual_block(n, width, hidden):
+    """Norm, two linear layers with the residual, backward through all, clipping, Adam: every stage against 64 bits on its own inputs."""
+    from neus2_amd.layers import GradientClip
+    from neus2_amd.tcnn_api import Adam
+    gen = torch.Generator().manual_seed(n)
+    block = Block(gen, width, hidden)
+    adam, clip = Adam(block.master, block.master.numel()), GradientClip([block.grads[s] for s in block.slices])
+    x, g = _rows(gen, n, width, torch.float16), _rows(gen, n, width, torch.float16, scale=128.0 / n)
+    for _ in range(2):
+        out, saved = block.forward(x)
+        _, y, ctx, h, z = saved
+        p = [block.params[s] for s in block.slices]
+        w1, b1 = p[1][:width * hidden].view(hidden, width), p[1][width * hidden:]
+        w2, b2 = p[2][:width * hidden].view(width, hidden), p[2][width * hidden:]
+        ref.within(y, *ref.norm_forward(x, p[0][:width], p[0][width:], 1e-5)[0], "norm")
+        he, ze, dh_, dz_ = ref.linear_forward(y, w1, b1, None, "GELU")
+        ref.within(h, he, dh_, "hidden")
+        oe, _, do_, _ = ref.linear_forward(h, w2, b2, x, "None")
+        ref.within(out, oe, do_, "out")
+        dx, dh, dy = block.backward(saved, g)
+        e2, e1 = ref.linear_backward(h, w2, None, g, "None"), ref.linear_backward(y, w1, z, dh, "GELU")
+        e0 = ref.norm_backward(x, *ctx, p[0][:width], dy, g)
+        for what, got, e in (("dh", dh, e2["dx"]), ("dy", dy, e1["dx"]), ("dx", dx, e0["dx"])):
+            ref.within(got, *e, what)
+        grads = [block.grads[s] for s in block.slices]
+        for what, got, e in (("dw2", grads[2][:-width].view(width, hidden), e2["dw"]), ("db2", grads[2][-width:], e2["db"]), ("dw1", grads[1][:-hidden].view(hidden, width), e1["dw"]),
+                             ("db1", grads[1][-hidden:], e1["db"]), ("dscale", grads[0][:width], e0["dscale"]), ("dshift", grads[0][width:], e0["dshift"])):
+            ref.within(got, *e, what)
+        before, exact = block.grads.clone(), float(block.grads.double().norm()) / 128
+        assert float(clip.clip(0.5 * exact, loss_scale=128.0)) == pytest.approx(exact, rel=10 * ref.U32)
+        ref.within(block.grads, before.double() * 0.5, before.double().abs() * 0.5 * (12 * ref.U32 + 1e-6 / exact), "clipped")
+        old = block.master.clone()
+        adam.step(block.params, block.grads)
+        assert bool((block.master != old).any()) and torch.equal(block.params, block.master.half())
+
+
+def test_a_captured_step_of_a_residual_block_replays():
+    """Forward, backward and clipping in a graph: every replay on new inputs gives what the eager calls give, with eager work between."""
+    from neus2_amd.layers import GradientClip
+    gen = torch.Generator().manual_seed(12)
+    block = Block(gen, 64, 192)
+    clip = GradientClip([block.grads])
+    x, g = _rows(gen, 500, 64, torch.float16), _rows(gen, 500, 64, torch.float16, scale=0.25)
+
+    def step():
+        out, saved = block.forward(x)
+        dx, _, _ = block.backward(saved, g)
+        return out, dx, clip.clip(0.01, loss_scale=128.0)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(4):
+        x.copy_(_rows(gen, 500, 64, torch.float16))
+        eager = [t.clone() for t in step()] + [block.grads.clone()]
+        block.grads.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip([*captured, block.grads], eager)), k
+
+
+def test_two_streams_at_once():
+    """Calls of one layer's shape on two streams at the same time, each with its own parameters' gradients."""
+    gen = torch.Generator().manual_seed(13)
+    pairs = []
+    for _ in range(2):
+        op, w, b = _linear(gen, 160, 96, "SiLU", bias=True, dtype=torch.float16)
+        pairs.append((op, _rows(gen, 3000, 160, torch.float16), _rows(gen, 3000, 96, torch.float16), _rows(gen, 3000, 96, torch.float16)))
+    alone = []
+    for op, x, z, dy in pairs:
+        alone.append((op.backward(x, z, dy), op._grads.clone()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for op, *_ in pairs:
+        op._grads.zero_()
+    torch.cuda.synchronize()
+    together = []
+    for _ in range(3):
+        for s, (op, x, z, dy) in zip(streams, pairs):
+            with torch.cuda.stream(s):
+                together.append(op.backward(x, z, dy))
+    torch.cuda.synchronize()
+    for k, (op, *_) in enumerate(pairs):
+        assert torch.equal(op._grads, alone[k][1])
+        assert all(torch.equal(t, alone[k][0]) for t in together[k::2])
