@@ -276,7 +276,7 @@ static inline uint32_t n2_layer_norm_blocks(uint32_t n_rows, uint32_t rows_per_b
 	return needed < most ? needed : most;
 }
 
-static inline uint32_t n2_ceil_div(uint64_t n, uint32_t by) { return (uint32_t)((n + by - 1u) / by); }
+N2_HD inline uint32_t n2_ceil_div(uint64_t n, uint32_t by) { return (uint32_t)((n + by - 1u) / by); }
 
 // Workgroups along the rows of a linear layer's pass over dz, each leaving a row of column sums.
 static inline uint32_t n2_linear_sum_blocks(uint32_t n_rows, uint32_t out_width) {
@@ -290,10 +290,24 @@ struct N2LinearSplit {
 	uint32_t splits, rows;
 };
 static inline N2LinearSplit n2_linear_gradient_split(uint32_t n_rows, uint32_t in_width, uint32_t out_width) {
-	const uint64_t tiles = (uint64_t)n2_ceil_div(in_width, 128u) * n2_ceil_div(out_width, 128u);
-	const uint64_t most = n2_ceil_div(n_rows, 256u), wanted = 512u / tiles;
+	const uint64_t tiles = (uint64_t)n2_ceil_div(in_width, 256u) * n2_ceil_div(out_width, 256u);
+	const uint64_t most = n2_ceil_div(n_rows, 256u), wanted = 256u / tiles;
 	const uint64_t splits = wanted < most ? wanted : most;
 	if (splits <= 1) return {1, n_rows};
 	const uint32_t rows = n2_ceil_div(n2_ceil_div(n_rows, (uint32_t)splits), 64u) * 64u;
 	return {n2_ceil_div(n_rows, rows), rows};
+}
+
+// Workgroups that come one after the other go to the XCDs in turn: the number that makes consecutive work one XCD's, which then reads it
+// from its own L2.
+N2_HD inline uint32_t n2_xcd_order(uint32_t block, uint32_t blocks) {
+	const uint32_t xcd = block % N2_XCDS, share = blocks / N2_XCDS, more = blocks % N2_XCDS;
+	return xcd * share + (xcd < more ? xcd : more) + block / N2_XCDS;
+}
+// Tiles of a product in groups of four rows of tiles, column by column: 32 consecutive ones, what an XCD's CUs take at a time, read four
+// tiles of one operand and eight of the other.
+N2_HD inline void n2_tile_order(uint32_t tile, uint32_t tiles_m, uint32_t tiles_n, uint32_t& m, uint32_t& n) {
+	const uint32_t group = tile / (4u * tiles_n), first = group * 4u, rows = tiles_m - first < 4u ? tiles_m - first : 4u, at = tile - first * tiles_n;
+	n = at / rows;
+	m = first + at - n * rows;
 }

@@ -52,7 +52,7 @@ struct Operand {
 template <bool KC, uint32_t R, uint32_t RUN>
 __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
 	if constexpr (KC) {
-		// the 16 rows of a fragment: consecutive ones, or four runs of four that stand RUN apart
+		// the 16 rows of a fragment: consecutive ones, or four runs of four that stand eight apart
 		const uint32_t f = RUN == 4u ? row % 8u : row % 4u + row / RUN % 2u * 4u;
 		return row * (BK / 8u) + (piece ^ f);
 	} else {
@@ -83,26 +83,39 @@ __device__ __forceinline__ void load_tile(uint4* __restrict__ lds, const Operand
 	}
 }
 
-// One operand of a matrix instruction: 16 indices by 32 values of k, lane l holding index l % 16 and the eight values from 8 * (l / 16) on.
-// The 16 indices are base + (i / 4) * RUN + i % 4.
+// Reads operands of matrix instructions: 16 indices by 32 values of k, lane l holding index l % 16 and the eight values from 8 * (l / 16)
+// on.  The 16 indices are consecutive (RUN 4), or four runs of four, eight apart (RUN 8); number u begins at first + b_base(u).  The
+// permutation of place() is the same for every u and kk, so a lane's address is one offset (two, for contiguous k) and constants.
+template <uint32_t RUN>
+__device__ __forceinline__ constexpr uint32_t b_base(uint32_t u) { return RUN == 4u ? u * 16u : u / 2u * 32u + u % 2u * 4u; }
+
 template <bool KC, uint32_t R, uint32_t RUN>
-__device__ __forceinline__ s16x8 fragment(const uint4* lds, uint32_t base, uint32_t kk) {
-	const uint32_t lane = threadIdx.x & 63u, i = lane % 16u, g = lane / 16u;
-	if constexpr (KC) {
-		return __builtin_bit_cast(s16x8, lds[place<KC, R, RUN>(base + i / 4u * RUN + i % 4u, kk * 4u + g)]);
-	} else {
-		static_assert(RUN == 4u, "");
-		typedef __attribute__((address_space(3))) s16x4* Half;
-		s16x8 r;
+struct Fragments {
+	uint32_t offset[KC ? BK / 32u : 1u];  // bytes
+
+	__device__ __forceinline__ explicit Fragments(uint32_t first) {
+		const uint32_t lane = threadIdx.x & 63u, i = lane % 16u, g = lane / 16u;
+		if constexpr (KC) {
 #pragma unroll
-		for (uint32_t h = 0; h < 2u; ++h) {
-			const uint32_t k = kk * 32u + g * 8u + h * 4u + i / 4u, m = base + i % 4u * 4u;
-			const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Half)(reinterpret_cast<const s16x4*>(lds + place<KC, R, RUN>(k, m / 8u)) + m / 4u % 2u));
-			r[h * 4 + 0] = v[0], r[h * 4 + 1] = v[1], r[h * 4 + 2] = v[2], r[h * 4 + 3] = v[3];
+			for (uint32_t kk = 0; kk < BK / 32u; ++kk) offset[kk] = 16u * place<KC, R, RUN>(first + i / 4u * RUN + i % 4u, kk * 4u + g);
+		} else {
+			static_assert(RUN == 4u, "");
+			offset[0] = 16u * place<KC, R, RUN>(g * 8u + i / 4u, first / 8u + i % 4u / 2u) + i % 2u * 8u;
 		}
-		return r;
 	}
-}
+	__device__ __forceinline__ s16x8 read(const uint4* tile, uint32_t u, uint32_t kk) const {
+		const char* lds = reinterpret_cast<const char*>(tile);
+		if constexpr (KC) {
+			return *reinterpret_cast<const s16x8*>(lds + offset[kk] + b_base<RUN>(u) * BK * 2u);
+		} else {
+			// (16 indices on: two pieces, whose number's bits the first one leaves free; four and 32 values of k on: rows of the same permutation)
+			typedef __attribute__((address_space(3))) s16x4* Half;
+			const char* p = lds + (offset[0] ^ u * 32u) + kk * 64u * R;
+			const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Half)(p)), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Half)(p + 8u * R));
+			return s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+		}
+	}
+};
 
 // -------------------------------------------------------------------------------------------------------------------------------------
 // the product
@@ -112,6 +125,7 @@ enum Epilogue { LAYER, STORE, GRADIENT, PARTIAL };
 struct Product {
 	Operand a, b;
 	uint32_t m, n, k;
+	uint32_t extent_a, extent_b;  // indices that may be read (of an operand contiguous in them a multiple of eight)
 	uint32_t tiles_m, tiles_n, k_per_split;
 	void* c;              // T [m][n], PARTIAL: fp32 [splits][m][n]
 	uint64_t ldc;
@@ -126,51 +140,71 @@ struct Product {
 };
 
 template <typename T, uint32_t N>
-__device__ __forceinline__ void store_run(T* p, const float (&v)[N], uint32_t valid) {
-	T t[N];
-#pragma unroll
-	for (uint32_t i = 0; i < N; ++i) t[i] = (T)v[i];
-	if (valid >= N) {
-		__builtin_memcpy(p, t, sizeof(t));
-	} else {
-#pragma unroll
-		for (uint32_t i = 0; i < N; ++i)
-			if (i < valid) p[i] = t[i];
-	}
-}
-template <typename T, uint32_t N>
-__device__ __forceinline__ void add_run(float (&v)[N], const T* p, uint32_t valid) {
-	T t[N];
-	if (valid >= N) {
-		__builtin_memcpy(t, p, sizeof(t));
-#pragma unroll
-		for (uint32_t i = 0; i < N; ++i) v[i] += (float)t[i];
-	} else {
-#pragma unroll
-		for (uint32_t i = 0; i < N; ++i)
-			if (i < valid) v[i] += (float)p[i];
-	}
-}
-
-// N consecutive values of row m from column n on
+struct Run {
+	T v[N];
+};
+// N consecutive values of row m from column n on, all of them inside
 template <typename T, int EPI, uint32_t N>
 __device__ __forceinline__ void finish(const Product& q, uint32_t m, uint32_t n, uint32_t split, float (&v)[N]) {
-	if (m >= q.m || n >= q.n) return;
-	const uint32_t valid = min(q.n - n, N);
+	auto add = [&](const T* p) __attribute__((always_inline)) {
+		Run<T, N> t;
+		__builtin_memcpy(&t, p, sizeof(t));
+#pragma unroll
+		for (uint32_t i = 0; i < N; ++i) v[i] += (float)t.v[i];
+	};
+	auto store = [&](auto* p) __attribute__((always_inline)) {
+		Run<std::remove_pointer_t<decltype(p)>, N> t;
+#pragma unroll
+		for (uint32_t i = 0; i < N; ++i) t.v[i] = (std::remove_pointer_t<decltype(p)>)v[i];
+		__builtin_memcpy(p, &t, sizeof(t));
+	};
 	if constexpr (EPI == PARTIAL) {
-		store_run(static_cast<float*>(q.c) + ((uint64_t)split * q.m + m) * q.n + n, v, valid);
+		store(static_cast<float*>(q.c) + ((uint64_t)split * q.m + m) * q.n + n);
 	} else {
 		T* c = static_cast<T*>(q.c) + (uint64_t)m * q.ldc + n;
 		if constexpr (EPI == LAYER) {
-			if (q.bias != nullptr) add_run(v, static_cast<const T*>(q.bias) + n, valid);
-			if (q.pre != nullptr) store_run(static_cast<T*>(q.pre) + (uint64_t)m * q.ldp + n, v, valid);
+			if (q.bias != nullptr) add(static_cast<const T*>(q.bias) + n);
+			if (q.pre != nullptr) store(static_cast<T*>(q.pre) + (uint64_t)m * q.ldp + n);
+			if (q.activation != N2_ACTIVATION_NONE)
 #pragma unroll
-			for (uint32_t i = 0; i < N; ++i) v[i] = activation(v[i], q.activation);
-			if (q.residual != nullptr) add_run(v, static_cast<const T*>(q.residual) + (uint64_t)m * q.ldr + n, valid);
+				for (uint32_t i = 0; i < N; ++i) v[i] = activation(v[i], q.activation);
+			if (q.residual != nullptr) add(static_cast<const T*>(q.residual) + (uint64_t)m * q.ldr + n);
 		}
 		if constexpr (EPI == GRADIENT)
-			if (q.accumulate) add_run(v, c, valid);
-		store_run(c, v, valid);
+			if (q.accumulate) add(c);
+		store(c);
+	}
+}
+
+// What a wave has of C, from (m0, n0) on.  Inside C a lane stores its runs of RUN columns; at an edge sixteen rows at a time go through
+// 4 KiB of LDS of the wave's own and are finished one by one, a row's columns side by side in the lanes.
+template <typename T, int EPI, uint32_t RUN, uint32_t S, uint32_t U>
+__device__ __forceinline__ void finish_all(const Product& q, uint32_t m0, uint32_t n0, uint32_t split, const f32x4 (&acc)[S][U], float* lds) {
+	static_assert(U == 4u, "");
+	const uint32_t lane = threadIdx.x & 63u;
+	if (m0 + S * 16u <= q.m && n0 + U * 16u <= q.n) {
+#pragma unroll
+		for (uint32_t s = 0; s < S; ++s)
+#pragma unroll
+			for (uint32_t u = 0; u < U; u += RUN / 4u) {
+				float v[RUN];
+#pragma unroll
+				for (uint32_t r = 0; r < RUN; ++r) v[r] = acc[s][u + r / 4u][r % 4u];
+				finish<T, EPI>(q, m0 + s * 16u + lane % 16u, n0 + b_base<RUN>(u) + lane / 16u * RUN, split, v);
+			}
+		return;
+	}
+#pragma unroll
+	for (uint32_t s = 0; s < S; ++s) {
+#pragma unroll
+		for (uint32_t u = 0; u < U; ++u) *reinterpret_cast<f32x4*>(lds + lane % 16u * 64u + (b_base<RUN>(u) + lane / 16u * RUN)) = acc[s][u];
+		__builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+		for (uint32_t row = 0; row < 16u; ++row) {
+			float v[1] = {lds[row * 64u + lane]};
+			if (m0 + s * 16u + row < q.m && n0 + lane < q.n) finish<T, EPI>(q, m0 + s * 16u + row, n0 + lane, split, v);
+		}
+		__builtin_amdgcn_wave_barrier();
 	}
 }
 
@@ -178,12 +212,14 @@ __device__ __forceinline__ void finish(const Product& q, uint32_t m, uint32_t n,
 // by side in a row of C; where B is contiguous in k its rows are dealt to the instructions so that all of a lane's values do.
 template <typename T, bool A_KC, bool B_KC, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, int EPI>
 __global__ void __launch_bounds__(WM* WN * 64) product_kernel(Product q) {
-	constexpr uint32_t THREADS = WM * WN * 64u, S = BM / WM / 16u, U = BN / WN / 16u, RUN = B_KC ? 4u * U : 4u;
+	constexpr uint32_t THREADS = WM * WN * 64u, S = BM / WM / 16u, U = BN / WN / 16u, RUN = B_KC ? 8u : 4u;
 	__shared__ uint4 tile_a[BM * BK / 8u], tile_b[BN * BK / 8u];
 	const uint32_t tile = blockIdx.x % (q.tiles_m * q.tiles_n), split = blockIdx.x / (q.tiles_m * q.tiles_n);
 	const uint32_t m0 = tile / q.tiles_n * BM, n0 = tile % q.tiles_n * BN;
 	const uint32_t wave = threadIdx.x / 64u, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
 	const uint32_t k_begin = split * q.k_per_split, k_end = min(q.k, k_begin + q.k_per_split);
+	const Fragments<A_KC, BM, 4u> a_read(wm);
+	const Fragments<B_KC, BN, RUN> b_read(wn);
 	f32x4 acc[S][U] = {};
 	for (uint32_t k0 = k_begin; k0 < k_end; k0 += BK) {
 		load_tile<T, A_KC, BM, 4u, THREADS>(tile_a, q.a, m0, q.m, k0, k_end);
@@ -193,9 +229,9 @@ __global__ void __launch_bounds__(WM* WN * 64) product_kernel(Product q) {
 		for (uint32_t kk = 0; kk < BK / 32u; ++kk) {
 			s16x8 a[S], b[U];
 #pragma unroll
-			for (uint32_t s = 0; s < S; ++s) a[s] = fragment<A_KC, BM, 4u>(tile_a, wm + s * 16u, kk);
+			for (uint32_t s = 0; s < S; ++s) a[s] = a_read.read(tile_a, s, kk);
 #pragma unroll
-			for (uint32_t u = 0; u < U; ++u) b[u] = fragment<B_KC, BN, RUN>(tile_b, wn + u * (B_KC ? 4u : 16u), kk);
+			for (uint32_t u = 0; u < U; ++u) b[u] = b_read.read(tile_b, u, kk);
 #pragma unroll
 			for (uint32_t s = 0; s < S; ++s)
 #pragma unroll
@@ -203,25 +239,110 @@ __global__ void __launch_bounds__(WM* WN * 64) product_kernel(Product q) {
 		}
 		__syncthreads();
 	}
-	const uint32_t lane = threadIdx.x & 63u;
+	finish_all<T, EPI, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a) + threadIdx.x / 64u * 1024u);
+}
+
+// The tile of load_tile straight from memory into LDS (no register in between): 16 bytes from each lane's address go to the wave's place and
+// 16 bytes times the lane, so a lane asks for the piece that belongs there.  Rows and pieces past the extent are the last ones once more; what
+// is computed from them is not stored.  Pieces past the end of k (a multiple of eight, for an operand contiguous in k) are zeros from g_zeros.
+__device__ const uint4 g_zeros = {0u, 0u, 0u, 0u};
+
+template <typename T, bool KC, uint32_t R, uint32_t RUN, uint32_t THREADS>
+struct AsyncTile {
+	static constexpr uint32_t LOADS = R * BK / 8u / THREADS, ROW = KC ? BK / 8u : R / 8u;
+	uint32_t offset[LOADS], k_of;  // (k_of: the lane's first k in a tile; KC: the same for all loads)
+	const char* base;
+	uint64_t step;
+
+	__device__ __forceinline__ AsyncTile(const Operand& o, uint32_t first, uint32_t extent, uint32_t k0) {
+		const T* p = static_cast<const T*>(o.p);
+		base = reinterpret_cast<const char*>(KC ? p + (uint64_t)first * o.ld + k0 : p + (uint64_t)k0 * o.ld + first);
+		step = (KC ? (uint64_t)BK : BK * o.ld) * sizeof(T);
+		static_assert(!KC || THREADS / ROW % 16u == 0u, "the permutation of place() repeats from load to load");
+		k_of = KC ? place<KC, R, RUN>(threadIdx.x / ROW, threadIdx.x % ROW) % ROW * 8u : threadIdx.x / ROW;
 #pragma unroll
-	for (uint32_t s = 0; s < S; ++s) {
-		const uint32_t m = m0 + wm + s * 16u + lane % 16u;
-		if constexpr (B_KC) {
-			float v[4u * U];
-#pragma unroll
-			for (uint32_t u = 0; u < U; ++u)
-#pragma unroll
-				for (uint32_t r = 0; r < 4u; ++r) v[u * 4u + r] = acc[s][u][r];
-			finish<T, EPI>(q, m, n0 + wn + lane / 16u * RUN, split, v);
-		} else {
-#pragma unroll
-			for (uint32_t u = 0; u < U; ++u) {
-				float v[4] = {acc[s][u][0], acc[s][u][1], acc[s][u][2], acc[s][u][3]};
-				finish<T, EPI>(q, m, n0 + wn + u * 16u + lane / 16u * 4u, split, v);
-			}
+		for (uint32_t i = 0; i < LOADS; ++i) {
+			const uint32_t at = i * THREADS + threadIdx.x, row = at / ROW, piece = place<KC, R, RUN>(row, at % ROW) % ROW;
+			offset[i] = KC ? min(row, extent - 1u - first) * (uint32_t)o.ld * 2u + piece * 16u : row * (uint32_t)o.ld * 2u + min(piece, (extent - first) / 8u - 1u) * 16u;
 		}
 	}
+	// left: values of k from this tile's first on, none included
+	__device__ __forceinline__ void load(uint4* lds, uint32_t i, uint32_t left) {
+		const char* from = k_of + (KC ? 0u : i * (THREADS / ROW)) < left ? base + offset[i] : reinterpret_cast<const char*>(&g_zeros);
+		__builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)(lds + i * THREADS + (threadIdx.x & ~63u)), 16, 0, 0);
+	}
+	__device__ __forceinline__ void advance() { base += step; }
+};
+
+// One stage of the product, in ta and tb, while the next one, of which `left` values of k are left, goes to next_a and next_b.  The matrix
+// instructions come in steps of U, one fragment of A each, which is read two steps ahead; B's fragments of the second half are read while
+// the first is computed; a load of the next stage is sent off with each step.  (That the four tiles do not overlap has to stand here: where
+// the compiler takes a load into LDS for one that a later reading meets, it waits for all loads before that.)
+template <typename T, bool A_KC, bool B_KC, uint32_t BM, uint32_t BN, uint32_t RUN, uint32_t THREADS, uint32_t S, uint32_t U>
+__device__ __forceinline__ void product_stage(const uint4* __restrict__ ta, const uint4* __restrict__ tb, uint4* __restrict__ next_a, uint4* __restrict__ next_b, uint32_t left,
+                                              const Fragments<A_KC, BM, 4u>& a_read, const Fragments<B_KC, BN, RUN>& b_read, AsyncTile<T, A_KC, BM, 4u, THREADS>& a_tile,
+                                              AsyncTile<T, B_KC, BN, RUN, THREADS>& b_tile, f32x4 (&acc)[S][U]) {
+	constexpr uint32_t STEPS = S * BK / 32u, AHEAD = 2u, LOADS_A = AsyncTile<T, A_KC, BM, 4u, THREADS>::LOADS, LOADS_B = AsyncTile<T, B_KC, BN, RUN, THREADS>::LOADS;
+	static_assert(BK == 64u && S >= U + AHEAD && LOADS_A + LOADS_B <= STEPS, "");
+	s16x8 a[STEPS], b[2][U];
+#pragma unroll
+	for (uint32_t u = 0; u < U; ++u) b[0][u] = b_read.read(tb, u, 0u);
+#pragma unroll
+	for (uint32_t i = 0; i < AHEAD; ++i) a[i] = a_read.read(ta, i, 0u);
+#pragma unroll
+	for (uint32_t i = 0; i < STEPS; ++i) {
+		constexpr uint32_t B_FROM = S - U - AHEAD;
+		if (i + AHEAD < STEPS) a[i + AHEAD] = a_read.read(ta, (i + AHEAD) % S, (i + AHEAD) / S);
+		if (i >= B_FROM && i < B_FROM + U) b[1][i - B_FROM] = b_read.read(tb, i - B_FROM, 1u);
+		if (i < LOADS_A) a_tile.load(next_a, i, left);
+		else if (i < LOADS_A + LOADS_B) b_tile.load(next_b, i - LOADS_A, left);
+#pragma unroll
+		for (uint32_t u = 0; u < U; ++u) acc[i % S][u] = mfma(T{}, b[i / S][u], a[i], acc[i % S][u]);
+		__builtin_amdgcn_sched_barrier(0);
+	}
+	a_tile.advance(), b_tile.advance();
+}
+
+// Two stages in LDS, 128 KiB, and eight waves of 128 x 64: a CU's LDS reads 96 of its 128 bytes a clock under full matrix cores.
+template <typename T, bool A_KC, bool B_KC, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, int EPI>
+__global__ void __launch_bounds__(WM* WN * 64) product_async_kernel(Product q) {
+	constexpr uint32_t THREADS = WM * WN * 64u, S = BM / WM / 16u, U = BN / WN / 16u, RUN = B_KC ? 8u : 4u;
+	__shared__ uint4 tile_a0[BM * BK / 8u], tile_a1[BM * BK / 8u], tile_b0[BN * BK / 8u], tile_b1[BN * BK / 8u];
+	const uint32_t tiles = q.tiles_m * q.tiles_n, work = n2_xcd_order(blockIdx.x, gridDim.x), split = work / tiles;
+	uint32_t tm, tn;
+	n2_tile_order(work - split * tiles, q.tiles_m, q.tiles_n, tm, tn);
+	const uint32_t m0 = tm * BM, n0 = tn * BN;
+	const uint32_t wave = threadIdx.x / 64u, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+	const uint32_t k_begin = split * q.k_per_split, k_end = min(q.k, k_begin + q.k_per_split);
+	AsyncTile<T, A_KC, BM, 4u, THREADS> a_tile(q.a, m0, q.extent_a, k_begin);
+	AsyncTile<T, B_KC, BN, RUN, THREADS> b_tile(q.b, n0, q.extent_b, k_begin);
+	const Fragments<A_KC, BM, 4u> a_read(wm);
+	const Fragments<B_KC, BN, RUN> b_read(wn);
+	f32x4 acc[S][U] = {};
+	uint32_t left = k_end - k_begin;  // values of k from the stage on that is asked for next
+	const uint32_t stages = n2_ceil_div(left, BK);
+	if (left > 0u) {
+#pragma unroll
+		for (uint32_t i = 0; i < a_tile.LOADS; ++i) a_tile.load(tile_a0, i, left);
+#pragma unroll
+		for (uint32_t i = 0; i < b_tile.LOADS; ++i) b_tile.load(tile_b0, i, left);
+		a_tile.advance(), b_tile.advance();
+	}
+	// (stages come in pairs: a branch out between the two would have the sums in other registers there)
+	for (uint32_t pair = 0; pair < stages / 2u; ++pair) {
+		left -= BK;
+		__syncthreads();
+		product_stage<T, A_KC, B_KC, BM, BN, RUN, THREADS>(tile_a0, tile_b0, tile_a1, tile_b1, left, a_read, b_read, a_tile, b_tile, acc);
+		left -= min(left, BK);
+		__syncthreads();
+		product_stage<T, A_KC, B_KC, BM, BN, RUN, THREADS>(tile_a1, tile_b1, tile_a0, tile_b0, left, a_read, b_read, a_tile, b_tile, acc);
+	}
+	if (stages % 2u != 0u) {
+		__syncthreads();
+		product_stage<T, A_KC, B_KC, BM, BN, RUN, THREADS>(tile_a0, tile_b0, tile_a1, tile_b1, 0u, a_read, b_read, a_tile, b_tile, acc);
+	}
+	__syncthreads();
+	finish_all<T, EPI, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a0) + wave * 1024u);
 }
 
 // -------------------------------------------------------------------------------------------------------------------------------------
@@ -264,13 +385,31 @@ __global__ void __launch_bounds__(256) slope_kernel(uint32_t n_rows, uint32_t wi
 	}
 }
 
+// an operand that can go into LDS without registers: pieces of 16 bytes at multiples of 16 bytes, offsets of a tile within 32 bits
+bool async_operand(const Operand& o, bool kc, uint32_t extent, uint32_t k) {
+	return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % 8 == 0 && o.ld < (1u << 22) && (kc ? k : extent) % 8 == 0;
+}
+
 template <typename T, bool A_KC, bool B_KC, int EPI>
 int launch_product(hipStream_t s, Product q, uint32_t splits, uint32_t k_per_split) {
-	constexpr uint32_t BM = 128, BN = 128;
-	q.tiles_m = n2_ceil_div(q.m, BM), q.tiles_n = n2_ceil_div(q.n, BN), q.k_per_split = k_per_split;
-	const uint64_t blocks = (uint64_t)q.tiles_m * q.tiles_n * splits;
-	N2_REQUIRE(blocks <= 0xFFFFFFFFull / 256u, "n2_linear: %u x %u values take %llu workgroups", q.m, q.n, (unsigned long long)blocks);
-	product_kernel<T, A_KC, B_KC, BM, BN, 2, 2, EPI><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(q);
+	q.k_per_split = k_per_split;
+	if (q.extent_a == 0) q.extent_a = q.m;
+	if (q.extent_b == 0) q.extent_b = q.n;
+	auto tiles = [&](uint32_t bm, uint32_t bn, uint32_t& blocks) -> int {
+		q.tiles_m = n2_ceil_div(q.m, bm), q.tiles_n = n2_ceil_div(q.n, bn);
+		const uint64_t all = (uint64_t)q.tiles_m * q.tiles_n * splits;
+		N2_REQUIRE(all <= 0xFFFFFFFFull / 512u, "n2_linear: %u x %u values take %llu workgroups", q.m, q.n, (unsigned long long)all);
+		blocks = (uint32_t)all;
+		return N2_OK;
+	};
+	uint32_t blocks = 0;
+	if (async_operand(q.a, A_KC, q.extent_a, q.k) && async_operand(q.b, B_KC, q.extent_b, q.k)) {
+		if (const int rc = tiles(256, 256, blocks)) return rc;
+		product_async_kernel<T, A_KC, B_KC, 256, 256, 2, 4, EPI><<<dim3(blocks), dim3(512), 0, s>>>(q);
+	} else {
+		if (const int rc = tiles(128, 128, blocks)) return rc;
+		product_kernel<T, A_KC, B_KC, 128, 128, 2, 2, EPI><<<dim3(blocks), dim3(256), 0, s>>>(q);
+	}
 	N2_LAUNCH_CHECK();
 	return N2_OK;
 }
