@@ -3,10 +3,6 @@
 #pragma once
 #include "layer_types.h"
 
-// 16 columns (64 bytes of a row) by 64 rows to a workgroup: with up to 1024 rows every lane has at most sixteen loads, all under way
-// at once, and what the launch takes is its latency.
-constexpr uint32_t N2_SUM_COLUMNS = 16, N2_SUM_ROWS = 64;
-
 // A run of columns of the partial sums and where their sums go.
 struct N2ColumnOutput {
 	void* out;           // [columns] of dtype, or null: nothing is stored
@@ -18,28 +14,62 @@ __device__ __forceinline__ void n2_store_sum(P* out, float sum, int accumulate) 
 	*out = (P)(accumulate ? (float)*out + sum : sum);
 }
 
-// partial: [rows][pitch]; the outputs' columns do not overlap
-template <int N_OUT>
-__global__ void __launch_bounds__(N2_SUM_COLUMNS* N2_SUM_ROWS) n2_column_sums_kernel(const float* __restrict__ partial, uint32_t rows, uint64_t pitch, uint32_t columns,
-                                                                                      N2ColumnOutput first, N2ColumnOutput second, int accumulate) {
-	__shared__ float part[N2_SUM_ROWS][N2_SUM_COLUMNS + 1];
-	const uint32_t x = threadIdx.x % N2_SUM_COLUMNS, y = threadIdx.x / N2_SUM_COLUMNS, column = blockIdx.x * N2_SUM_COLUMNS + x;
-	float sum = 0.f;
-	if (column < columns) {
+// partial: [rows][columns]; the outputs' columns follow each other.  A workgroup takes LANES * WIDE columns by ROWS rows.
+template <int N_OUT, uint32_t LANES, uint32_t WIDE, uint32_t ROWS>
+__global__ void __launch_bounds__(LANES* ROWS) n2_column_sums_kernel(const float* __restrict__ partial, uint32_t rows, uint32_t columns, N2ColumnOutput first, N2ColumnOutput second,
+                                                                      int accumulate) {
+	__shared__ float part[ROWS > 1u ? ROWS : 1u][LANES * WIDE + 1u];
+	const uint32_t x = threadIdx.x % LANES * WIDE, y = threadIdx.x / LANES, column = blockIdx.x * LANES * WIDE + x;
+	float sum[WIDE] = {};
+	const uint32_t valid = column < columns ? min(columns - column, WIDE) : 0u;
 #pragma unroll 16
-		for (uint32_t r = y; r < rows; r += N2_SUM_ROWS) sum += partial[r * pitch + column];
+	for (uint32_t r = y; r < rows; r += ROWS) {
+		float v[WIDE] = {};
+		const float* p = partial + (uint64_t)r * columns + column;
+		if (valid == WIDE) {
+			__builtin_memcpy(v, p, sizeof(v));
+		} else {
+#pragma unroll
+			for (uint32_t i = 0; i < WIDE; ++i) v[i] = i < valid ? p[i] : 0.f;
+		}
+#pragma unroll
+		for (uint32_t i = 0; i < WIDE; ++i) sum[i] += v[i];
 	}
-	part[y][x] = sum;
-	__syncthreads();
-	for (uint32_t half = N2_SUM_ROWS / 2; half > 0; half /= 2) {
-		if (y < half) part[y][x] += part[y + half][x];
+	if constexpr (ROWS > 1u) {
+#pragma unroll
+		for (uint32_t i = 0; i < WIDE; ++i) part[y][x + i] = sum[i];
 		__syncthreads();
+		for (uint32_t half = ROWS / 2u; half > 0u; half /= 2u) {
+			if (y < half)
+#pragma unroll
+				for (uint32_t i = 0; i < WIDE; ++i) part[y][x + i] += part[y + half][x + i];
+			__syncthreads();
+		}
+		if (y != 0u) return;
+#pragma unroll
+		for (uint32_t i = 0; i < WIDE; ++i) sum[i] = part[0][x + i];
 	}
-	if (y != 0 || column >= columns) return;
-	const N2ColumnOutput o = N_OUT > 1 && column >= second.first ? second : first;
-	if (o.out == nullptr || column < o.first || column >= o.first + o.columns) return;
-	const uint32_t at = column - o.first;
-	if (o.dtype == N2_DTYPE_F16) n2_store_sum(static_cast<n2_f16*>(o.out) + at, part[0][x], accumulate);
-	else if (o.dtype == N2_DTYPE_BF16) n2_store_sum(static_cast<n2_bf16*>(o.out) + at, part[0][x], accumulate);
-	else n2_store_sum(static_cast<float*>(o.out) + at, part[0][x], accumulate);
+#pragma unroll
+	for (uint32_t i = 0; i < WIDE; ++i) {
+		if (i >= valid) break;
+		const N2ColumnOutput o = N_OUT > 1 && column + i >= second.first ? second : first;
+		const uint32_t at = column + i - o.first;
+		if (o.dtype == N2_DTYPE_F16) n2_store_sum(static_cast<n2_f16*>(o.out) + at, sum[i], accumulate);
+		else if (o.dtype == N2_DTYPE_BF16) n2_store_sum(static_cast<n2_bf16*>(o.out) + at, sum[i], accumulate);
+		else n2_store_sum(static_cast<float*>(o.out) + at, sum[i], accumulate);
+	}
+}
+
+// Few columns: 64 bytes of a row by 64 rows to a workgroup, with up to 1024 rows at most sixteen loads to a lane, all under way at once; the
+// launch takes its latency.  Many columns: 16 bytes a lane, sixteen rows at a time; few rows of them: a lane takes its columns' sums alone.
+template <int N_OUT>
+static inline int n2_column_sums(hipStream_t s, const float* partial, uint32_t rows, uint32_t columns, const N2ColumnOutput& first, const N2ColumnOutput& second, int accumulate) {
+	if (rows <= 16u && columns >= 4096u)
+		n2_column_sums_kernel<N_OUT, 256, 4, 1><<<dim3(n2_ceil_div(columns, 1024u)), dim3(256), 0, s>>>(partial, rows, columns, first, second, accumulate);
+	else if (columns >= 16384u)
+		n2_column_sums_kernel<N_OUT, 16, 4, 16><<<dim3(n2_ceil_div(columns, 64u)), dim3(256), 0, s>>>(partial, rows, columns, first, second, accumulate);
+	else
+		n2_column_sums_kernel<N_OUT, 16, 1, 64><<<dim3(n2_ceil_div(columns, 16u)), dim3(1024), 0, s>>>(partial, rows, columns, first, second, accumulate);
+	N2_LAUNCH_CHECK();
+	return N2_OK;
 }

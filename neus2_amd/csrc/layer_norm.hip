@@ -290,8 +290,5 @@ N2_API int n2_layer_norm_backward(n2_stream_t stream, n2_dtype dtype, n2_dtype w
 	}
 	if (!weights) return N2_OK;
 	const N2ColumnOutput scale_out = {d_dL_dscale, 0, width, (uint32_t)weights_dtype}, shift_out = {d_dL_dshift, width, width, (uint32_t)weights_dtype};
-	n2_column_sums_kernel<2><<<dim3((2u * width + N2_SUM_COLUMNS - 1u) / N2_SUM_COLUMNS), dim3(N2_SUM_COLUMNS * N2_SUM_ROWS), 0, s>>>(
-		static_cast<const float*>(d_workspace), blocks, 2ull * width, 2u * width, scale_out, shift_out, mode == N2_GRAD_ACCUMULATE ? 1 : 0);
-	N2_LAUNCH_CHECK();
-	return N2_OK;
+	return n2_column_sums<2>(s, static_cast<const float*>(d_workspace), blocks, 2u * width, scale_out, shift_out, mode == N2_GRAD_ACCUMULATE ? 1 : 0);
 }

@@ -540,14 +540,12 @@ N2_API int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation 
 				if (const int rc = launch_product<T, false, false, PARTIAL>(s, q, p.splits, p.k_per_split)) return rc;
 				const uint64_t n = (uint64_t)in_width * out_width;
 				const N2ColumnOutput out = {dw, 0, (uint32_t)n, (uint32_t)dtype};
-				n2_column_sums_kernel<1><<<dim3((uint32_t)((n + N2_SUM_COLUMNS - 1) / N2_SUM_COLUMNS)), dim3(N2_SUM_COLUMNS * N2_SUM_ROWS), 0, s>>>(partial, p.splits, n, (uint32_t)n, out, out, accumulate);
-				N2_LAUNCH_CHECK();
+				if (const int rc = n2_column_sums<1>(s, partial, p.splits, (uint32_t)n, out, out, accumulate)) return rc;
 			}
 		}
 		if (db != nullptr) {
 			const N2ColumnOutput out = {db, 0, out_width, (uint32_t)dtype};
-			n2_column_sums_kernel<1><<<dim3(n2_ceil_div(out_width, N2_SUM_COLUMNS)), dim3(N2_SUM_COLUMNS * N2_SUM_ROWS), 0, s>>>(sums, n_rows > 0 ? p.sum_blocks : 0u, out_width, out_width, out, out, accumulate);
-			N2_LAUNCH_CHECK();
+			if (const int rc = n2_column_sums<1>(s, sums, n_rows > 0 ? p.sum_blocks : 0u, out_width, out, out, accumulate)) return rc;
 		}
 		return N2_OK;
 	});
