@@ -942,7 +942,8 @@ typedef enum n2_activation {
  *  d_bias            NULL or [out_width]
  *  d_residual        NULL or [n_rows][out_width]
  *  d_pre_activation  NULL or [n_rows][out_width], written: z, what the backward pass of an activation reads
- *  The activation is taken of z before it is rounded.  in_width and out_width are 1 to 65536.
+ *  The activation is taken of z before it is rounded.  in_width and out_width are 1 to 65536,
+ *  n_rows below 2^31.
  *  d_workspace       n2_linear_forward_workspace_bytes(n_rows, in_width, out_width) bytes (may be 0), 16-byte aligned */
 uint64_t n2_linear_forward_workspace_bytes(uint32_t n_rows, uint32_t in_width, uint32_t out_width);
 int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation activation, uint32_t n_rows, uint32_t in_width, uint32_t out_width,

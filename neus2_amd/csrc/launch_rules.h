@@ -280,23 +280,44 @@ N2_HD inline uint32_t n2_ceil_div(uint64_t n, uint32_t by) { return (uint32_t)((
 
 // Workgroups along the rows of a linear layer's pass over dz, each leaving a row of column sums.
 static inline uint32_t n2_linear_sum_blocks(uint32_t n_rows, uint32_t out_width) {
-	const uint32_t columns = n2_ceil_div(out_width, 512u), most = 1024u / columns > 16u ? 1024u / columns : 16u, needed = n2_ceil_div(n_rows, 4u);
+	const uint32_t lanes = out_width <= 64u ? 8u : out_width <= 128u ? 16u : out_width <= 256u ? 32u : 64u, columns = n2_ceil_div(out_width, lanes * 8u);
+	const uint32_t most = 1024u / columns > 16u ? 1024u / columns : 16u, needed = n2_ceil_div(n_rows, 256u / lanes);
 	return needed < most ? needed : most;
 }
 
-// The weights' gradient of a linear layer is a product over all rows: where its tiles are fewer than the CUs, the rows are dealt out to
-// several workgroups for each tile, which leave fp32 sums.
-struct N2LinearSplit {
-	uint32_t splits, rows;
+// How C [m][n] of a sum over k is cut: square tiles to a workgroup, and where those are fewer than the CUs k is dealt out to several
+// workgroups for each, which leave fp32 sums that a second launch joins.
+struct N2LinearPlan {
+	uint32_t tile, splits, k_per_split;
 };
-static inline N2LinearSplit n2_linear_gradient_split(uint32_t n_rows, uint32_t in_width, uint32_t out_width) {
-	const uint64_t tiles = (uint64_t)n2_ceil_div(in_width, 256u) * n2_ceil_div(out_width, 256u);
-	const uint64_t most = n2_ceil_div(n_rows, 256u), wanted = 256u / tiles;
-	const uint64_t splits = wanted < most ? wanted : most;
-	if (splits <= 1) return {1, n_rows};
-	const uint32_t rows = n2_ceil_div(n2_ceil_div(n_rows, (uint32_t)splits), 64u) * 64u;
-	return {n2_ceil_div(n_rows, rows), rows};
+static inline N2LinearPlan n2_linear_plan(uint32_t m, uint32_t n, uint32_t k) {
+	const auto tiles_of = [&](uint32_t t) { return (uint64_t)n2_ceil_div(m, t) * n2_ceil_div(n, t); };
+	const auto fits = [&](uint32_t t) { return 4u * t * t * tiles_of(t) <= 5ull * m * n; };  // at most a quarter of the tiles is past the edges
+	const auto split = [&](uint32_t tile, uint64_t wanted, uint64_t most) -> N2LinearPlan {
+		const uint64_t splits = wanted < most ? wanted : most;
+		if (splits <= 1) return {tile, 1, k};
+		const uint32_t rows = n2_ceil_div(n2_ceil_div(k, (uint32_t)splits), 64u) * 64u;
+		return {tile, n2_ceil_div(k, rows), rows};
+	};
+	if (m == 0 || n == 0 || k == 0) return {64, 1, k};
+	if (fits(256) && tiles_of(256) >= 192 && k >= 512) return {256, 1, k};
+	if (fits(128) && tiles_of(128) >= 1024) return {128, 1, k};
+	if (fits(256) && tiles_of(64) >= 1024 && k >= 4096) return split(256, 256u / tiles_of(256), k / 640u);
+	if (fits(128) && k >= 16384) return split(128, 512u / tiles_of(128), k / 640u);
+	// small tiles: what a launch takes in us, 3 and 0.45 for a stage of 64 (times as many as do not run at once), and what joining takes
+	const uint32_t stages = n2_ceil_div(k, 64u);
+	const double tiles = (double)tiles_of(64);
+	uint32_t best = 1;
+	double least = 0.;
+	constexpr uint32_t tried[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
+	for (uint32_t s : tried) {
+		if (s > 1u && (2u * s > stages || tiles * s > 1024.)) break;
+		const double turns = tiles * s / 512., us = 0.45 * stages / s * (turns > 1. ? turns : 1.) + (s > 1u ? 2. + 0.06 * s + s * ((double)m * n) * 8. / 3e6 : 0.);
+		if (s == 1u || us < least) best = s, least = us;
+	}
+	return split(64, best, best);
 }
+static inline uint64_t n2_linear_partial_bytes(const N2LinearPlan& plan, uint32_t m, uint32_t n) { return plan.splits > 1 ? 4ull * plan.splits * m * n : 0ull; }
 
 // Workgroups that come one after the other go to the XCDs in turn: the number that makes consecutive work one XCD's, which then reads it
 // from its own L2.

@@ -45,6 +45,7 @@ constexpr uint32_t BK = 64;
 struct Operand {
 	const void* p;
 	uint64_t ld;
+	bool padded;  // what stands between a row's end and the next multiple of eight values is zero
 };
 
 // A tile of R indices by BK in LDS, 16 bytes (eight values) at a time.  Contiguous in k: R rows of eight pieces.  Contiguous in its own
@@ -176,13 +177,13 @@ __device__ __forceinline__ void finish(const Product& q, uint32_t m, uint32_t n,
 	}
 }
 
-// What a wave has of C, from (m0, n0) on.  Inside C a lane stores its runs of RUN columns; at an edge sixteen rows at a time go through
-// 4 KiB of LDS of the wave's own and are finished one by one, a row's columns side by side in the lanes.
+// What a wave has of C, from (m0, n0) on.  Inside C a lane stores its runs of RUN columns; at an edge sixteen rows at a time go through LDS
+// of the wave's own (16 rows of its columns) and are finished one by one, a row's columns side by side in the lanes.
 template <typename T, int EPI, uint32_t RUN, uint32_t S, uint32_t U>
 __device__ __forceinline__ void finish_all(const Product& q, uint32_t m0, uint32_t n0, uint32_t split, const f32x4 (&acc)[S][U], float* lds) {
-	static_assert(U == 4u, "");
+	constexpr uint32_t WIDTH = U * 16u;
 	const uint32_t lane = threadIdx.x & 63u;
-	if (m0 + S * 16u <= q.m && n0 + U * 16u <= q.n) {
+	if (m0 + S * 16u <= q.m && n0 + WIDTH <= q.n) {
 #pragma unroll
 		for (uint32_t s = 0; s < S; ++s)
 #pragma unroll
@@ -194,15 +195,18 @@ __device__ __forceinline__ void finish_all(const Product& q, uint32_t m0, uint32
 			}
 		return;
 	}
+	if (m0 >= q.m || n0 >= q.n) return;
+	float* mine = lds + threadIdx.x / 64u * 16u * WIDTH;
 #pragma unroll
 	for (uint32_t s = 0; s < S; ++s) {
 #pragma unroll
-		for (uint32_t u = 0; u < U; ++u) *reinterpret_cast<f32x4*>(lds + lane % 16u * 64u + (b_base<RUN>(u) + lane / 16u * RUN)) = acc[s][u];
+		for (uint32_t u = 0; u < U; ++u) *reinterpret_cast<f32x4*>(mine + lane % 16u * WIDTH + (b_base<RUN>(u) + lane / 16u * RUN)) = acc[s][u];
 		__builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-		for (uint32_t row = 0; row < 16u; ++row) {
-			float v[1] = {lds[row * 64u + lane]};
-			if (m0 + s * 16u + row < q.m && n0 + lane < q.n) finish<T, EPI>(q, m0 + s * 16u + row, n0 + lane, split, v);
+		for (uint32_t i = lane; i < 16u * WIDTH; i += 64u) {
+			const uint32_t m = m0 + s * 16u + i / WIDTH, n = n0 + i % WIDTH;
+			float v[1] = {mine[i]};
+			if (m < q.m && n < q.n) finish<T, EPI>(q, m, n, split, v);
 		}
 		__builtin_amdgcn_wave_barrier();
 	}
@@ -239,7 +243,7 @@ __global__ void __launch_bounds__(WM* WN * 64) product_kernel(Product q) {
 		}
 		__syncthreads();
 	}
-	finish_all<T, EPI, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a) + threadIdx.x / 64u * 1024u);
+	finish_all<T, EPI, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a));
 }
 
 // The tile of load_tile straight from memory into LDS (no register in between): 16 bytes from each lane's address go to the wave's place and
@@ -283,17 +287,23 @@ __device__ __forceinline__ void product_stage(const uint4* __restrict__ ta, cons
                                               const Fragments<A_KC, BM, 4u>& a_read, const Fragments<B_KC, BN, RUN>& b_read, AsyncTile<T, A_KC, BM, 4u, THREADS>& a_tile,
                                               AsyncTile<T, B_KC, BN, RUN, THREADS>& b_tile, f32x4 (&acc)[S][U]) {
 	constexpr uint32_t STEPS = S * BK / 32u, AHEAD = 2u, LOADS_A = AsyncTile<T, A_KC, BM, 4u, THREADS>::LOADS, LOADS_B = AsyncTile<T, B_KC, BN, RUN, THREADS>::LOADS;
-	static_assert(BK == 64u && S >= U + AHEAD && LOADS_A + LOADS_B <= STEPS, "");
+	// (smaller tiles read B's fragments of both halves at once)
+	constexpr bool BOTH = S < U + AHEAD;
+	static_assert(BK == 64u && LOADS_A + LOADS_B <= STEPS, "");
 	s16x8 a[STEPS], b[2][U];
 #pragma unroll
 	for (uint32_t u = 0; u < U; ++u) b[0][u] = b_read.read(tb, u, 0u);
 #pragma unroll
-	for (uint32_t i = 0; i < AHEAD; ++i) a[i] = a_read.read(ta, i, 0u);
+	for (uint32_t i = 0; i < AHEAD; ++i) a[i] = a_read.read(ta, i % S, i / S);
+	if constexpr (BOTH) {
+#pragma unroll
+		for (uint32_t u = 0; u < U; ++u) b[1][u] = b_read.read(tb, u, 1u);
+	}
 #pragma unroll
 	for (uint32_t i = 0; i < STEPS; ++i) {
-		constexpr uint32_t B_FROM = S - U - AHEAD;
+		constexpr uint32_t B_FROM = BOTH ? 0u : S - U - AHEAD;
 		if (i + AHEAD < STEPS) a[i + AHEAD] = a_read.read(ta, (i + AHEAD) % S, (i + AHEAD) / S);
-		if (i >= B_FROM && i < B_FROM + U) b[1][i - B_FROM] = b_read.read(tb, i - B_FROM, 1u);
+		if (!BOTH && i >= B_FROM && i < B_FROM + U) b[1][i - B_FROM] = b_read.read(tb, i - B_FROM, 1u);
 		if (i < LOADS_A) a_tile.load(next_a, i, left);
 		else if (i < LOADS_A + LOADS_B) b_tile.load(next_b, i - LOADS_A, left);
 #pragma unroll
@@ -342,23 +352,52 @@ __global__ void __launch_bounds__(WM* WN * 64) product_async_kernel(Product q) {
 		product_stage<T, A_KC, B_KC, BM, BN, RUN, THREADS>(tile_a0, tile_b0, tile_a1, tile_b1, 0u, a_read, b_read, a_tile, b_tile, acc);
 	}
 	__syncthreads();
-	finish_all<T, EPI, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a0) + wave * 1024u);
+	finish_all<T, EPI, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a0));
+}
+
+// The sums of the parts that k was dealt out to, [splits][m][n], finished: a lane takes four columns of a row.
+template <typename T, int EPI>
+__global__ void __launch_bounds__(256) join_kernel(Product q, const float* __restrict__ partial, uint32_t splits) {
+	const uint32_t quads = n2_ceil_div(q.n, 4u);
+	const uint64_t at = (uint64_t)blockIdx.x * 256u + threadIdx.x, row = at / quads;
+	if (row >= q.m) return;
+	const uint32_t m = (uint32_t)row, n = (uint32_t)(at - row * quads) * 4u, valid = min(q.n - n, 4u);
+	float v[4] = {0.f, 0.f, 0.f, 0.f};
+	const float* p = partial + row * q.n + n;
+	const uint64_t pitch = (uint64_t)q.m * q.n;
+	if (valid == 4u) {
+#pragma unroll 8
+		for (uint32_t i = 0; i < splits; ++i) {
+			float t[4];
+			__builtin_memcpy(t, p + i * pitch, 16);
+			v[0] += t[0], v[1] += t[1], v[2] += t[2], v[3] += t[3];
+		}
+		finish<T, EPI>(q, m, n, 0u, v);
+	} else {
+		for (uint32_t j = 0; j < valid; ++j) {
+			float w[1] = {0.f};
+			for (uint32_t i = 0; i < splits; ++i) w[0] += p[i * pitch + j];
+			finish<T, EPI>(q, m, n + j, 0u, w);
+		}
+	}
 }
 
 // -------------------------------------------------------------------------------------------------------------------------------------
 // dz = dy * act'(z), and its column sums
 // -------------------------------------------------------------------------------------------------------------------------------------
-// A workgroup takes 64 * VEC columns and rows gridDim.y * 4 apart, a wave a row at a time.  dz (or null) goes into rows of ld_dz values, a
-// multiple of eight, zero behind the width; partial (or null): one row of sums from each workgroup.
-template <typename T>
+// LANES lanes of eight values take a row (512 columns of it, where it is wider), rows as far apart as the launch has groups of lanes along
+// them.  dz (or null) goes into rows of ld_dz values, a multiple of eight, zero behind the width; partial (or null): one row of sums from
+// each workgroup.
+template <typename T, uint32_t LANES>
 __global__ void __launch_bounds__(256) slope_kernel(uint32_t n_rows, uint32_t width, const T* __restrict__ dy, uint64_t ld_dy, const T* __restrict__ z, uint64_t ld_z, int kind,
                                                     T* __restrict__ dz, uint64_t ld_dz, float* __restrict__ partial) {
-	constexpr uint32_t VEC = N2Vec<T>::SIZE;
-	const uint32_t column = (blockIdx.x * 64u + threadIdx.x % 64u) * VEC, wave = threadIdx.x / 64u;
+	constexpr uint32_t VEC = N2Vec<T>::SIZE, ROWS = 256u / LANES, COLUMNS = LANES * VEC;
+	const uint32_t lane = threadIdx.x % LANES, column = blockIdx.x * COLUMNS + lane * VEC, group = threadIdx.x / LANES;
 	const uint32_t n = n2_left<T>(width, column);
 	float sum[VEC] = {};
 	if (column < width) {
-		for (uint64_t row = blockIdx.y * 4u + wave; row < n_rows; row += gridDim.y * 4u) {
+#pragma unroll 4
+		for (uint64_t row = (uint64_t)blockIdx.y * ROWS + group; row < n_rows; row += (uint64_t)gridDim.y * ROWS) {
 			const N2Vec<T> g = n2_load_vec(dy + row * ld_dy + column, n);
 			N2Vec<T> out = {}, pre = {};
 			if (kind != N2_ACTIVATION_NONE) pre = n2_load_vec(z + row * ld_z + column, n);
@@ -375,40 +414,55 @@ __global__ void __launch_bounds__(256) slope_kernel(uint32_t n_rows, uint32_t wi
 		}
 	}
 	if (partial == nullptr) return;
-	__shared__ float fold[4][64 * VEC];
+	__shared__ float fold[ROWS][COLUMNS + 4u];
 #pragma unroll
-	for (uint32_t i = 0; i < VEC; ++i) fold[wave][threadIdx.x % 64u * VEC + i] = sum[i];
+	for (uint32_t i = 0; i < VEC; ++i) fold[group][lane * VEC + i] = sum[i];
 	__syncthreads();
-	for (uint32_t i = threadIdx.x; i < 64u * VEC; i += 256u) {
-		const uint32_t at = blockIdx.x * 64u * VEC + i;
-		if (at < width) partial[(uint64_t)blockIdx.y * width + at] = (fold[0][i] + fold[1][i]) + (fold[2][i] + fold[3][i]);
+	for (uint32_t i = threadIdx.x; i < COLUMNS; i += 256u) {
+		const uint32_t at = blockIdx.x * COLUMNS + i;
+		float s = 0.f;
+#pragma unroll
+		for (uint32_t r = 0; r < ROWS; ++r) s += fold[r][i];
+		if (at < width) partial[(uint64_t)blockIdx.y * width + at] = s;
 	}
 }
 
 // an operand that can go into LDS without registers: pieces of 16 bytes at multiples of 16 bytes, offsets of a tile within 32 bits
 bool async_operand(const Operand& o, bool kc, uint32_t extent, uint32_t k) {
-	return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % 8 == 0 && o.ld < (1u << 22) && (kc ? k : extent) % 8 == 0;
+	return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % 8 == 0 && o.ld < (1u << 22) && (o.padded || (kc ? k : extent) % 8 == 0);
 }
 
+// C by the plan; partial: n2_linear_partial_bytes of it
 template <typename T, bool A_KC, bool B_KC, int EPI>
-int launch_product(hipStream_t s, Product q, uint32_t splits, uint32_t k_per_split) {
-	q.k_per_split = k_per_split;
+int launch_product(hipStream_t s, Product q, const N2LinearPlan& plan, float* partial) {
+	q.k_per_split = plan.k_per_split;
 	if (q.extent_a == 0) q.extent_a = q.m;
 	if (q.extent_b == 0) q.extent_b = q.n;
-	auto tiles = [&](uint32_t bm, uint32_t bn, uint32_t& blocks) -> int {
-		q.tiles_m = n2_ceil_div(q.m, bm), q.tiles_n = n2_ceil_div(q.n, bn);
-		const uint64_t all = (uint64_t)q.tiles_m * q.tiles_n * splits;
-		N2_REQUIRE(all <= 0xFFFFFFFFull / 512u, "n2_linear: %u x %u values take %llu workgroups", q.m, q.n, (unsigned long long)all);
-		blocks = (uint32_t)all;
-		return N2_OK;
+	q.tiles_m = n2_ceil_div(q.m, plan.tile), q.tiles_n = n2_ceil_div(q.n, plan.tile);
+	const uint64_t blocks = (uint64_t)q.tiles_m * q.tiles_n * plan.splits;
+	N2_REQUIRE(blocks <= 0xFFFFFFFFull / 512u, "n2_linear: %u x %u values take %llu workgroups", q.m, q.n, (unsigned long long)blocks);
+	auto launch = [&](auto epi, const Product& p) {
+		constexpr int E = decltype(epi)::value;
+		const dim3 grid((uint32_t)blocks);
+		if (async_operand(q.a, A_KC, q.extent_a, q.k) && async_operand(q.b, B_KC, q.extent_b, q.k)) {
+			if (plan.tile == 256) product_async_kernel<T, A_KC, B_KC, 256, 256, 2, 4, E><<<grid, dim3(512), 0, s>>>(p);
+			else if (plan.tile == 128) product_async_kernel<T, A_KC, B_KC, 128, 128, 2, 2, E><<<grid, dim3(256), 0, s>>>(p);
+			else product_async_kernel<T, A_KC, B_KC, 64, 64, 2, 2, E><<<grid, dim3(256), 0, s>>>(p);
+		} else {
+			if (plan.tile == 256) product_kernel<T, A_KC, B_KC, 256, 256, 2, 4, E><<<grid, dim3(512), 0, s>>>(p);
+			else if (plan.tile == 128) product_kernel<T, A_KC, B_KC, 128, 128, 2, 2, E><<<grid, dim3(256), 0, s>>>(p);
+			else product_kernel<T, A_KC, B_KC, 64, 64, 2, 2, E><<<grid, dim3(256), 0, s>>>(p);
+		}
 	};
-	uint32_t blocks = 0;
-	if (async_operand(q.a, A_KC, q.extent_a, q.k) && async_operand(q.b, B_KC, q.extent_b, q.k)) {
-		if (const int rc = tiles(256, 256, blocks)) return rc;
-		product_async_kernel<T, A_KC, B_KC, 256, 256, 2, 4, EPI><<<dim3(blocks), dim3(512), 0, s>>>(q);
+	if (plan.splits <= 1) {
+		launch(std::integral_constant<int, EPI>{}, q);
 	} else {
-		if (const int rc = tiles(128, 128, blocks)) return rc;
-		product_kernel<T, A_KC, B_KC, 128, 128, 2, 2, EPI><<<dim3(blocks), dim3(256), 0, s>>>(q);
+		Product part = q;
+		part.c = partial;
+		launch(std::integral_constant<int, PARTIAL>{}, part);
+		N2_LAUNCH_CHECK();
+		const uint64_t lanes = (uint64_t)q.m * n2_ceil_div(q.n, 4u);
+		join_kernel<T, EPI><<<dim3((uint32_t)((lanes + 255u) / 256u)), dim3(256), 0, s>>>(q, partial, plan.splits);
 	}
 	N2_LAUNCH_CHECK();
 	return N2_OK;
@@ -424,7 +478,8 @@ constexpr uint32_t MAX_WIDTH = 65536;
 // what a backward pass keeps in its workspace, in this order
 struct BackwardPlan {
 	uint64_t ld_dz, dz_bytes, sums_bytes, partial_bytes;
-	uint32_t sum_blocks, splits, k_per_split;
+	uint32_t sum_blocks;
+	N2LinearPlan input, weights;
 };
 BackwardPlan backward_plan(uint32_t n_rows, uint32_t in_width, uint32_t out_width) {
 	BackwardPlan p = {};
@@ -432,9 +487,10 @@ BackwardPlan backward_plan(uint32_t n_rows, uint32_t in_width, uint32_t out_widt
 	p.dz_bytes = (n_rows * p.ld_dz * 2u + 15u) / 16u * 16u;
 	p.sum_blocks = n2_linear_sum_blocks(n_rows, out_width);
 	p.sums_bytes = ((uint64_t)p.sum_blocks * out_width * 4u + 15u) / 16u * 16u;
-	const N2LinearSplit split = n2_linear_gradient_split(n_rows, in_width, out_width);
-	p.splits = split.splits, p.k_per_split = split.rows;
-	p.partial_bytes = p.splits > 1 ? (uint64_t)p.splits * in_width * out_width * 4u : 0u;
+	p.input = n2_linear_plan(n_rows, in_width, out_width);
+	p.weights = n2_linear_plan(out_width, in_width, n_rows);
+	const uint64_t a = n2_linear_partial_bytes(p.input, n_rows, in_width), b = n2_linear_partial_bytes(p.weights, out_width, in_width);
+	p.partial_bytes = a > b ? a : b;
 	return p;
 }
 
@@ -443,11 +499,14 @@ BackwardPlan backward_plan(uint32_t n_rows, uint32_t in_width, uint32_t out_widt
 #define LINEAR_CHECKS(name)                                                                                                                                \
 	N2_REQUIRE(dtype == N2_DTYPE_F16 || dtype == N2_DTYPE_BF16, name ": type %d is neither fp16 nor bf16", (int)dtype);                                    \
 	N2_REQUIRE((int)activation >= N2_ACTIVATION_NONE && (int)activation <= N2_ACTIVATION_GELU, name ": activation %d", (int)activation);                   \
-	N2_REQUIRE(in_width >= 1 && in_width <= MAX_WIDTH && out_width >= 1 && out_width <= MAX_WIDTH, name ": widths %u, %u outside [1, %u]", in_width, out_width, MAX_WIDTH)
+	N2_REQUIRE(in_width >= 1 && in_width <= MAX_WIDTH && out_width >= 1 && out_width <= MAX_WIDTH, name ": widths %u, %u outside [1, %u]", in_width, out_width, MAX_WIDTH); \
+	N2_REQUIRE(n_rows < (1u << 31), name ": %u rows, 2^31 - 1 are the most", n_rows)
 #define STRIDE_CHECK(name, what, pointer, stride, width) \
 	N2_REQUIRE((pointer) == nullptr || n_rows <= 1 || ((stride) >= (width) && n2_rows_fit(n_rows, stride)), name ": the stride of " what " is below the width %u or beyond memory", width)
 
-N2_API uint64_t n2_linear_forward_workspace_bytes(uint32_t n_rows, uint32_t in_width, uint32_t out_width) { return 0; }
+N2_API uint64_t n2_linear_forward_workspace_bytes(uint32_t n_rows, uint32_t in_width, uint32_t out_width) {
+	return n_rows == 0 || in_width == 0 || out_width == 0 ? 0u : n2_linear_partial_bytes(n2_linear_plan(n_rows, out_width, in_width), n_rows, out_width);
+}
 
 N2_API int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation activation, uint32_t n_rows, uint32_t in_width, uint32_t out_width, const void* d_weights,
                              const void* d_bias, const void* d_input, uint64_t input_stride, const void* d_residual, uint64_t residual_stride, void* d_output, uint64_t output_stride,
@@ -468,11 +527,11 @@ N2_API int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation a
 	                        n2_rows(in_place ? nullptr : d_residual, n_rows, out_width, residual_stride, 2)};
 	N2_REQUIRE(!n2_overlap(written, read), "n2_linear_forward: an output overlaps another buffer");
 	Product q = {};
-	q.a = {d_input, input_stride}, q.b = {d_weights, in_width};
+	q.a = {d_input, input_stride, false}, q.b = {d_weights, in_width, false};
 	q.m = n_rows, q.n = out_width, q.k = in_width;
 	q.c = d_output, q.ldc = output_stride;
 	q.bias = d_bias, q.residual = d_residual, q.ldr = residual_stride, q.pre = d_pre_activation, q.ldp = pre_stride, q.activation = activation;
-	return with_type(dtype, [&](auto t) { return launch_product<decltype(t), true, true, LAYER>(n2_stream(stream), q, 1, in_width); });
+	return with_type(dtype, [&](auto t) { return launch_product<decltype(t), true, true, LAYER>(n2_stream(stream), q, n2_linear_plan(n_rows, out_width, in_width), static_cast<float*>(d_workspace)); });
 }
 
 N2_API uint64_t n2_linear_backward_workspace_bytes(uint32_t n_rows, uint32_t in_width, uint32_t out_width) {
@@ -512,36 +571,37 @@ N2_API int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation 
 	float* const partial = reinterpret_cast<float*>(ws + p.dz_bytes + p.sums_bytes);
 	return with_type(dtype, [&](auto t) -> int {
 		using T = decltype(t);
-		// dz: the output's gradient itself where there is no activation
-		const bool products = d_dL_dinput != nullptr || dw != nullptr, writes = activation != N2_ACTIVATION_NONE && products;
-		Operand dz = {d_dL_doutput, dL_doutput_stride};
+		// dz: the output's gradient itself where there is no activation and its rows can go into LDS as they are
+		const bool products = d_dL_dinput != nullptr || dw != nullptr, aligned = reinterpret_cast<uintptr_t>(d_dL_doutput) % 16 == 0 && dL_doutput_stride % 8 == 0 && out_width % 8 == 0;
+		const bool writes = products && (activation != N2_ACTIVATION_NONE || !aligned);
+		Operand dz = {d_dL_doutput, dL_doutput_stride, false};
 		if (n_rows > 0 && (writes || db != nullptr)) {
-			if (writes) dz = {ws, p.ld_dz};
-			slope_kernel<T><<<dim3(n2_ceil_div(out_width, 512u), p.sum_blocks), dim3(256), 0, s>>>(n_rows, out_width, static_cast<const T*>(d_dL_doutput), dL_doutput_stride,
-				static_cast<const T*>(d_pre_activation), pre_stride, activation, writes ? reinterpret_cast<T*>(ws) : nullptr, p.ld_dz, db != nullptr ? sums : nullptr);
+			if (writes) dz = {ws, p.ld_dz, true};
+			auto launch = [&](auto lanes) {
+				constexpr uint32_t LANES = decltype(lanes)::value;
+				slope_kernel<T, LANES><<<dim3(n2_ceil_div(out_width, LANES * 8u), p.sum_blocks), dim3(256), 0, s>>>(n_rows, out_width, static_cast<const T*>(d_dL_doutput), dL_doutput_stride,
+					static_cast<const T*>(d_pre_activation), pre_stride, activation, writes ? reinterpret_cast<T*>(ws) : nullptr, p.ld_dz, db != nullptr ? sums : nullptr);
+			};
+			if (out_width <= 64u) launch(std::integral_constant<uint32_t, 8>{});
+			else if (out_width <= 128u) launch(std::integral_constant<uint32_t, 16>{});
+			else if (out_width <= 256u) launch(std::integral_constant<uint32_t, 32>{});
+			else launch(std::integral_constant<uint32_t, 64>{});
 			N2_LAUNCH_CHECK();
 		}
 		if (d_dL_dinput != nullptr && n_rows > 0) {
 			Product q = {};
-			q.a = dz, q.b = {d_weights, in_width};
+			q.a = dz, q.b = {d_weights, in_width, false};
 			q.m = n_rows, q.n = in_width, q.k = out_width;
 			q.c = d_dL_dinput, q.ldc = dL_dinput_stride;
-			if (const int rc = launch_product<T, true, false, STORE>(s, q, 1, out_width)) return rc;
+			if (const int rc = launch_product<T, true, false, STORE>(s, q, p.input, partial)) return rc;
 		}
 		if (dw != nullptr) {
 			Product q = {};
-			q.a = dz, q.b = {d_input, input_stride};
+			q.a = dz, q.b = {d_input, input_stride, false};
 			q.m = out_width, q.n = in_width, q.k = n_rows;
+			if (dz.padded) q.extent_a = (uint32_t)p.ld_dz;
 			q.c = dw, q.ldc = in_width, q.accumulate = accumulate;
-			if (p.splits <= 1) {
-				if (const int rc = launch_product<T, false, false, GRADIENT>(s, q, 1, n_rows)) return rc;
-			} else {
-				q.c = partial;
-				if (const int rc = launch_product<T, false, false, PARTIAL>(s, q, p.splits, p.k_per_split)) return rc;
-				const uint64_t n = (uint64_t)in_width * out_width;
-				const N2ColumnOutput out = {dw, 0, (uint32_t)n, (uint32_t)dtype};
-				if (const int rc = n2_column_sums<1>(s, partial, p.splits, (uint32_t)n, out, out, accumulate)) return rc;
-			}
+			if (const int rc = launch_product<T, false, false, GRADIENT>(s, q, p.weights, partial)) return rc;
 		}
 		if (db != nullptr) {
 			const N2ColumnOutput out = {db, 0, out_width, (uint32_t)dtype};

@@ -30,8 +30,8 @@ def _matrix(t, dtype, rows, width, what):
     shape = t.shape
     if t.dtype != dtype or len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows):
         raise N2Error(f"{what} must be a {dtype} tensor [{'N' if rows is None else rows}, {width}], got {t.dtype} {tuple(shape)}")
-    if shape[0] >= 1 << 32:
-        raise N2Error(f"{what} has {shape[0]} rows, 2^32 - 1 are the most")
+    if shape[0] >= 1 << 31:
+        raise N2Error(f"{what} has {shape[0]} rows, 2^31 - 1 are the most")
     if t.numel() == 0:
         return width
     stride, inner = t.stride()

@@ -45,7 +45,7 @@ def norm_backward(dtype=0, weights=0, n=64, w=32, scale=A, x=B, xs=None, mean=D,
 
 def test_linear_forward_refuses():
     accepted(linear(n=0, x=0, y=0))
-    for kw, text in ((dict(dtype=2), "neither"), (dict(dtype=7), "neither"), (dict(act=4), "activation"), (dict(act=-1), "activation"), (dict(i=0), "widths"), (dict(o=0), "widths"), (dict(i=65537), "widths"),
+    for kw, text in ((dict(dtype=2), "neither"), (dict(dtype=7), "neither"), (dict(act=4), "activation"), (dict(act=-1), "activation"), (dict(i=0), "widths"), (dict(o=0), "widths"), (dict(i=65537), "widths"), (dict(n=1 << 31), "rows"),
                      (dict(w=0), "null"), (dict(x=0), "null"), (dict(y=0), "null"), (dict(xs=31), "the input"), (dict(ys=47), "the output"), (dict(r=E, rs=40), "residual"),
                      (dict(z=E, zs=1), "saved"), (dict(xs=1 << 61), "the input"),
                      (dict(y=B), "overlaps"), (dict(y=A), "overlaps"), (dict(y=B + 64 * 64 - 2), "overlaps"), (dict(z=D), "overlaps"), (dict(z=B), "overlaps"), (dict(r=D, rs=50), "overlaps"),
