@@ -270,9 +270,15 @@ static inline N2GatherGrid n2_rows_of_blocks(uint32_t blocks, uint32_t threads) 
 	return {(x + N2_XCDS - 1u) / N2_XCDS * N2_XCDS, y};
 }
 
-// Workgroups of a layer norm's launch, each taking groups of rows as far apart as there are workgroups.
-static inline uint32_t n2_layer_norm_blocks(uint32_t n_rows, uint32_t rows_per_block, uint32_t threads) {
-	const uint32_t needed = n_rows / rows_per_block + (n_rows % rows_per_block != 0u), most = threads > 256u ? 512u : 1024u;
+// Workgroups of a layer norm's launch, each taking groups of rows as far apart as there are workgroups.  Backward, where each leaves two rows
+// of fp32 sums: at least eight rows to one beyond the first 256.
+static inline uint32_t n2_layer_norm_forward_blocks(uint32_t n_rows, uint32_t rows_per_block, uint32_t threads) {
+	const uint32_t needed = n_rows / rows_per_block + (n_rows % rows_per_block != 0u), most = threads > 256u ? 512u : 2048u;
+	return needed < most ? needed : most;
+}
+static inline uint32_t n2_layer_norm_backward_blocks(uint32_t n_rows, uint32_t rows_per_block, uint32_t threads) {
+	const uint32_t needed = n_rows / rows_per_block + (n_rows % rows_per_block != 0u), top = threads > 256u ? 512u : 1024u;
+	const uint32_t some = n_rows / 8u > 256u ? n_rows / 8u : 256u, most = some < top ? some : top;
 	return needed < most ? needed : most;
 }
 

@@ -11,14 +11,16 @@ namespace {
 // LANES lanes share a row, each with CHUNKS vectors of it, LANES vectors apart.
 template <uint32_t LANES>
 constexpr uint32_t threads_of() { return LANES > 256u ? LANES : 256u; }
+// Rows that a lane has under way at once, so that memory is kept busy: forward four vectors of them, backward, which reads two or three
+// matrices, two.
+template <uint32_t LANES, uint32_t CHUNKS, bool BACKWARD>
+constexpr uint32_t rows_at_once() { return BACKWARD ? (LANES > 64u ? 1u : 2u) : LANES > 512u ? 1u : LANES > 256u ? 2u : 4u; }
 
-// sum over the lanes of a row, in all of them
+// sums over the lanes of a row, in all of them
 template <uint32_t LANES, uint32_t N>
 __device__ __forceinline__ void row_sums(float (&v)[N], float (*shared)[N]) {
 #pragma unroll
-	for (uint32_t o = min(LANES, 64u) / 2u; o > 0u; o /= 2u)
-#pragma unroll
-		for (uint32_t k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], (int)o);
+	for (uint32_t k = 0; k < N; ++k) v[k] = n2_lane_sum<(LANES < 64u ? LANES : 64u)>(v[k]);
 	if constexpr (LANES > 64u) {
 		constexpr uint32_t WAVES = LANES / 64u;
 		__syncthreads();  // (the sums before are read)
@@ -30,10 +32,17 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*shared)[N]) {
 		for (uint32_t k = 0; k < N; ++k) {
 			float s = 0.f;
 #pragma unroll
-			for (uint32_t w = 0; w < WAVES; ++w) s += shared[w][k];
+			for (uint32_t w = 0; w < WAVES; ++w) s += shared[threadIdx.x / LANES * WAVES + w][k];
 			v[k] = s;
 		}
 	}
+}
+
+template <typename T>
+__device__ __forceinline__ void as_loaded(N2Vec<T>& v) {
+	n2_u32x4 u = __builtin_bit_cast(n2_u32x4, v);
+	asm("" : "+v"(u));
+	v = __builtin_bit_cast(N2Vec<T>, u);
 }
 
 // sum / width to the last bit, where sum * (1 / width) is a step off: rows of equal values have no variance
@@ -42,137 +51,204 @@ __device__ __forceinline__ float mean_of(float sum, float width, float inv) {
 	return fmaf(fmaf(-m, width, sum), inv, m);
 }
 
+// a lane's weights, zero past the width
+template <typename P, uint32_t LANES, uint32_t CHUNKS, uint32_t VEC>
+struct Weights {
+	P v[CHUNKS][VEC];
+	__device__ __forceinline__ Weights(const P* __restrict__ p, uint32_t width, uint32_t lane) {
+#pragma unroll
+		for (uint32_t c = 0; c < CHUNKS; ++c) {
+			const uint32_t at = (c * LANES + lane) * VEC;
+			if (at + VEC <= width) {
+				__builtin_memcpy(v[c], p + at, sizeof(v[c]));
+			} else {
+#pragma unroll
+				for (uint32_t i = 0; i < VEC; ++i) v[c][i] = at + i < width ? p[at + i] : (P)0.f;
+			}
+		}
+	}
+};
+
 template <typename T, typename P, uint32_t LANES, uint32_t CHUNKS>
 __global__ void __launch_bounds__(threads_of<LANES>()) layer_norm_forward_kernel(uint32_t n_rows, uint32_t width, float epsilon, const P* __restrict__ scale, const P* __restrict__ shift,
                                                                                   const T* x, uint64_t x_stride, T* y, uint64_t y_stride, float* __restrict__ mean_out,
                                                                                   float* __restrict__ rstd_out) {
-	constexpr uint32_t VEC = N2Vec<T>::SIZE, ROWS = threads_of<LANES>() / LANES;
-	__shared__ float shared[LANES > 64u ? LANES / 64u : 1u][1];
-	const uint32_t lane = threadIdx.x % LANES;
+	constexpr uint32_t VEC = N2Vec<T>::SIZE, ROWS = threads_of<LANES>() / LANES, R = rows_at_once<LANES, CHUNKS, false>();
+	__shared__ float shared[LANES > 64u ? threads_of<LANES>() / 64u : 1u][R];
+	const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
 	const float inv = 1.f / (float)width;
-	for (uint64_t row = (uint64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row - threadIdx.x / LANES < n_rows; row += (uint64_t)gridDim.x * ROWS) {
-		const bool live = row < n_rows;  // (the lanes of a workgroup's last rows stay for the barriers)
-		float v[CHUNKS][VEC], sum[1] = {0.f};
+	const uint64_t end = (uint64_t)(n_rows - 1u) * x_stride + width;
+	const Weights<P, LANES, CHUNKS, VEC> g(scale, width, lane), b(shift, width, lane);
+	// (the lanes of a workgroup's last rows stay for the barriers)
+	for (uint64_t first = (uint64_t)blockIdx.x * ROWS * R; first < n_rows; first += (uint64_t)gridDim.x * ROWS * R) {
+		N2Vec<T> in[R][CHUNKS];
+		float sum[R], mean[R];
 #pragma unroll
-		for (uint32_t c = 0; c < CHUNKS; ++c) {
-			const uint32_t at = (c * LANES + lane) * VEC, n = live ? n2_left<T>(width, at) : 0u;
-			const N2Vec<T> in = n2_load_vec(x + row * x_stride + at, n);
+		for (uint32_t r = 0; r < R; ++r)
 #pragma unroll
-			for (uint32_t i = 0; i < VEC; ++i) v[c][i] = (float)in.v[i], sum[0] += v[c][i];
+			for (uint32_t c = 0; c < CHUNKS; ++c) {
+				const uint64_t row = first + r * ROWS + group;
+				const uint32_t at = (c * LANES + lane) * VEC;
+				in[r][c] = n2_load_row(x, row * x_stride + at, end, row < n_rows ? n2_left<T>(width, at) : 0u);
+			}
+#pragma unroll
+		for (uint32_t r = 0; r < R; ++r) {
+			sum[r] = 0.f;
+#pragma unroll
+			for (uint32_t c = 0; c < CHUNKS; ++c)
+#pragma unroll
+				for (uint32_t i = 0; i < VEC; ++i) sum[r] += (float)in[r][c].v[i];
 		}
 		row_sums<LANES>(sum, shared);
-		const float mean = mean_of(sum[0], (float)width, inv);
-		sum[0] = 0.f;
 #pragma unroll
-		for (uint32_t c = 0; c < CHUNKS; ++c) {
-			const uint32_t at = (c * LANES + lane) * VEC;
-#pragma unroll
-			for (uint32_t i = 0; i < VEC; ++i) {
-				v[c][i] = at + i < width ? v[c][i] - mean : 0.f;
-				sum[0] += v[c][i] * v[c][i];
-			}
-		}
-		row_sums<LANES>(sum, shared);
-		const float rstd = rsqrtf(sum[0] * inv + epsilon);
-		if (live && lane == 0u) {
-			if (mean_out != nullptr) mean_out[row] = mean;
-			if (rstd_out != nullptr) rstd_out[row] = rstd;
-		}
-#pragma unroll
-		for (uint32_t c = 0; c < CHUNKS; ++c) {
-			const uint32_t at = (c * LANES + lane) * VEC, n = live ? n2_left<T>(width, at) : 0u;
-			N2Vec<T> out;
-#pragma unroll
-			for (uint32_t i = 0; i < VEC; ++i) out.v[i] = i < n ? (T)(v[c][i] * rstd * (float)scale[at + i] + (float)shift[at + i]) : (T)0.f;
-			n2_store_vec(y + row * y_stride + at, out, n);
-		}
-	}
-}
-
-// Backward: a workgroup takes rows gridDim.x apart and keeps the weights' gradients of its columns in registers; each leaves one row of
-// fp32 sums, [blocks][2][width], for n2_column_sums_kernel.
-template <typename T, typename P, uint32_t LANES, uint32_t CHUNKS>
-__global__ void __launch_bounds__(threads_of<LANES>()) layer_norm_backward_kernel(uint32_t n_rows, uint32_t width, const P* __restrict__ scale, const T* __restrict__ x, uint64_t x_stride,
-                                                                                   const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ dy, uint64_t dy_stride,
-                                                                                   const T* skip, uint64_t skip_stride, T* dx, uint64_t dx_stride, float* __restrict__ partial) {
-	constexpr uint32_t VEC = N2Vec<T>::SIZE, THREADS = threads_of<LANES>(), ROWS = THREADS / LANES, COLUMNS = LANES * CHUNKS * VEC;
-	__shared__ float shared[LANES > 64u ? LANES / 64u : 1u][2];
-	const uint32_t lane = threadIdx.x % LANES;
-	const float inv = 1.f / (float)width;
-	float dscale[CHUNKS][VEC] = {}, dshift[CHUNKS][VEC] = {};
-	for (uint64_t row = (uint64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row - threadIdx.x / LANES < n_rows; row += (uint64_t)gridDim.x * ROWS) {
-		const bool live = row < n_rows;
-		const float m = live ? mean[row] : 0.f, r = live ? rstd[row] : 0.f;
-		float xh[CHUNKS][VEC], h[CHUNKS][VEC], sum[2] = {0.f, 0.f};
-#pragma unroll
-		for (uint32_t c = 0; c < CHUNKS; ++c) {
-			const uint32_t at = (c * LANES + lane) * VEC, n = live ? n2_left<T>(width, at) : 0u;
-			const N2Vec<T> in = n2_load_vec(x + row * x_stride + at, n), g = n2_load_vec(dy + row * dy_stride + at, n);
-#pragma unroll
-			for (uint32_t i = 0; i < VEC; ++i) {
-				xh[c][i] = i < n ? ((float)in.v[i] - m) * r : 0.f;
-				h[c][i] = (float)g.v[i];
-				dscale[c][i] += h[c][i] * xh[c][i];
-				dshift[c][i] += h[c][i];
-				h[c][i] *= i < n ? (float)scale[at + i] : 0.f;
-				sum[0] += h[c][i];
-				sum[1] += h[c][i] * xh[c][i];
-			}
-		}
-		if (dx == nullptr) continue;
-		row_sums<LANES>(sum, shared);
-		const float a = sum[0] * inv, b = sum[1] * inv;
-#pragma unroll
-		for (uint32_t c = 0; c < CHUNKS; ++c) {
-			const uint32_t at = (c * LANES + lane) * VEC, n = live ? n2_left<T>(width, at) : 0u;
-			N2Vec<T> out = {}, add = {};
-			if (skip != nullptr) add = n2_load_vec(skip + row * skip_stride + at, n);
-#pragma unroll
-			for (uint32_t i = 0; i < VEC; ++i) out.v[i] = (T)(r * (h[c][i] - a - xh[c][i] * b) + (float)add.v[i]);
-			n2_store_vec(dx + row * dx_stride + at, out, n);
-		}
-	}
-	if (partial == nullptr) return;
-	// the workgroup's rows of lanes, one after the other, in one row of sums
-	__shared__ float fold[ROWS > 1u ? COLUMNS : 1u];
-#pragma unroll
-	for (uint32_t k = 0; k < 2u; ++k) {
-		float(&mine)[CHUNKS][VEC] = k == 0u ? dscale : dshift;
-		if constexpr (ROWS > 1u) {
-			for (uint32_t turn = ROWS - 1u; turn > 0u; --turn) {
-				if (threadIdx.x / LANES == turn)
-#pragma unroll
-					for (uint32_t c = 0; c < CHUNKS; ++c)
-#pragma unroll
-						for (uint32_t i = 0; i < VEC; ++i) {
-							float& f = fold[(c * LANES + lane) * VEC + i];
-							f = turn == ROWS - 1u ? mine[c][i] : f + mine[c][i];
-						}
-				__syncthreads();
-			}
-		}
-		if (threadIdx.x / LANES == 0u)
+		for (uint32_t r = 0; r < R; ++r) {
+			mean[r] = mean_of(sum[r], (float)width, inv);
+			sum[r] = 0.f;
 #pragma unroll
 			for (uint32_t c = 0; c < CHUNKS; ++c)
 #pragma unroll
 				for (uint32_t i = 0; i < VEC; ++i) {
-					const uint32_t at = (c * LANES + lane) * VEC + i;
-					if (at < width) partial[((uint64_t)blockIdx.x * 2u + k) * width + at] = ROWS > 1u ? mine[c][i] + fold[at] : mine[c][i];
+					const float d = (c * LANES + lane) * VEC + i < width ? (float)in[r][c].v[i] - mean[r] : 0.f;
+					sum[r] += d * d;
 				}
-		if constexpr (ROWS > 1u) __syncthreads();
+		}
+		row_sums<LANES>(sum, shared);
+#pragma unroll
+		for (uint32_t r = 0; r < R; ++r) {
+			const uint64_t row = first + r * ROWS + group;
+			const float rstd = rsqrtf(sum[r] * inv + epsilon);
+			if (row < n_rows && lane == 0u) {
+				if (mean_out != nullptr) mean_out[row] = mean[r];
+				if (rstd_out != nullptr) rstd_out[row] = rstd;
+			}
+#pragma unroll
+			for (uint32_t c = 0; c < CHUNKS; ++c) {
+				const uint32_t at = (c * LANES + lane) * VEC;
+				N2Vec<T> out;
+#pragma unroll
+				for (uint32_t i = 0; i < VEC; ++i) out.v[i] = (T)(((float)in[r][c].v[i] - mean[r]) * rstd * (float)g.v[c][i] + (float)b.v[c][i]);
+				n2_store_vec(y + row * y_stride + at, out, row < n_rows ? n2_left<T>(width, at) : 0u);
+			}
+		}
+	}
+}
+
+// Backward: a workgroup takes groups of rows gridDim.x apart and keeps the weights' gradients of its columns in registers; each leaves one
+// row of fp32 sums, [blocks][2][width], for n2_column_sums.
+template <typename T, typename P, uint32_t LANES, uint32_t CHUNKS>
+__global__ void __launch_bounds__(threads_of<LANES>(), LANES <= 512u ? 4 : 1) layer_norm_backward_kernel(uint32_t n_rows, uint32_t width, const P* __restrict__ scale, const T* __restrict__ x, uint64_t x_stride,
+                                                                                   const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ dy, uint64_t dy_stride,
+                                                                                   const T* skip, uint64_t skip_stride, T* dx, uint64_t dx_stride, float* __restrict__ partial) {
+	constexpr uint32_t VEC = N2Vec<T>::SIZE, THREADS = threads_of<LANES>(), ROWS = THREADS / LANES, COLUMNS = LANES * CHUNKS * VEC, R = rows_at_once<LANES, CHUNKS, true>();
+	__shared__ float shared[LANES > 64u ? THREADS / 64u : 1u][2 * R];
+	const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+	const float inv = 1.f / (float)width;
+	const uint64_t end_x = (uint64_t)(n_rows - 1u) * x_stride + width, end_dy = (uint64_t)(n_rows - 1u) * dy_stride + width, end_skip = (uint64_t)(n_rows - 1u) * skip_stride + width;
+	const Weights<P, LANES, CHUNKS, VEC> w(scale, width, lane);
+	float dscale[CHUNKS][VEC] = {}, dshift[CHUNKS][VEC] = {};
+	for (uint64_t first = (uint64_t)blockIdx.x * ROWS * R; first < n_rows; first += (uint64_t)gridDim.x * ROWS * R) {
+		N2Vec<T> in[R][CHUNKS], g[R][CHUNKS], add[R][CHUNKS];
+		float m[R], s[R], sum[2 * R];
+#pragma unroll
+		for (uint32_t r = 0; r < R; ++r) {
+			const uint64_t row = first + r * ROWS + group;
+			const bool live = row < n_rows;
+			m[r] = live ? mean[row] : 0.f, s[r] = live ? rstd[row] : 0.f;
+#pragma unroll
+			for (uint32_t c = 0; c < CHUNKS; ++c) {
+				const uint32_t at = (c * LANES + lane) * VEC, n = live ? n2_left<T>(width, at) : 0u;
+				in[r][c] = n2_load_row(x, row * x_stride + at, end_x, n);
+				g[r][c] = n2_load_row(dy, row * dy_stride + at, end_dy, n);
+				add[r][c] = N2Vec<T>{};
+				if (skip != nullptr) add[r][c] = n2_load_row(skip, row * skip_stride + at, end_skip, n);
+			}
+		}
+#pragma unroll
+		for (uint32_t r = 0; r < R; ++r) {
+			sum[2 * r] = sum[2 * r + 1] = 0.f;
+#pragma unroll
+			for (uint32_t c = 0; c < CHUNKS; ++c)
+#pragma unroll
+				for (uint32_t i = 0; i < VEC; ++i) {
+					// (past the width, and for rows past the last, dy is zero and so is the scale)
+					const float xh = ((float)in[r][c].v[i] - m[r]) * s[r], d = (float)g[r][c].v[i], h = d * (float)w.v[c][i];
+					dscale[c][i] += d * xh;
+					dshift[c][i] += d;
+					sum[2 * r] += h;
+					sum[2 * r + 1] += h * xh;
+				}
+		}
+		if (dx == nullptr) continue;
+		row_sums<LANES>(sum, shared);
+		// (the second half takes the rows' values from the registers they came in: kept as fp32 they would halve the waves)
+		if constexpr (LANES <= 256u)
+#pragma unroll
+			for (uint32_t r = 0; r < R; ++r)
+#pragma unroll
+				for (uint32_t c = 0; c < CHUNKS; ++c) as_loaded(in[r][c]), as_loaded(g[r][c]);
+#pragma unroll
+		for (uint32_t r = 0; r < R; ++r) {
+			const uint64_t row = first + r * ROWS + group;
+			const float a = sum[2 * r] * inv, b = sum[2 * r + 1] * inv;
+#pragma unroll
+			for (uint32_t c = 0; c < CHUNKS; ++c) {
+				const uint32_t at = (c * LANES + lane) * VEC;
+				N2Vec<T> out;
+#pragma unroll
+				for (uint32_t i = 0; i < VEC; ++i) {
+					const float xh = ((float)in[r][c].v[i] - m[r]) * s[r], h = (float)g[r][c].v[i] * (float)w.v[c][i];
+					out.v[i] = (T)(s[r] * (h - a - xh * b) + (float)add[r][c].v[i]);
+				}
+				n2_store_vec(dx + row * dx_stride + at, out, row < n_rows ? n2_left<T>(width, at) : 0u);
+			}
+		}
+	}
+	if (partial == nullptr) return;
+	// the workgroup's groups of lanes in one row of sums: those of a wave by exchange, the waves through LDS
+	if constexpr (ROWS > 1u) {
+		constexpr uint32_t PARTS = LANES < 64u ? THREADS / 64u : ROWS;
+		__shared__ float fold[PARTS][COLUMNS];
+#pragma unroll
+		for (uint32_t k = 0; k < 2u; ++k) {
+			float(&mine)[CHUNKS][VEC] = k == 0u ? dscale : dshift;
+#pragma unroll
+			for (uint32_t c = 0; c < CHUNKS; ++c)
+#pragma unroll
+				for (uint32_t i = 0; i < VEC; ++i) {
+#pragma unroll
+					for (uint32_t o = LANES; o < 64u; o *= 2u) mine[c][i] += __shfl_xor(mine[c][i], (int)o);
+					if (threadIdx.x % 64u < LANES) fold[LANES < 64u ? threadIdx.x / 64u : group][(c * LANES + lane) * VEC + i] = mine[c][i];
+				}
+			__syncthreads();
+			for (uint32_t at = threadIdx.x; at < min(COLUMNS, width); at += THREADS) {
+				float sum = 0.f;
+#pragma unroll
+				for (uint32_t p = 0; p < PARTS; ++p) sum += fold[p][at];
+				partial[((uint64_t)blockIdx.x * 2u + k) * width + at] = sum;
+			}
+			__syncthreads();
+		}
+	} else {
+#pragma unroll
+		for (uint32_t c = 0; c < CHUNKS; ++c)
+#pragma unroll
+			for (uint32_t i = 0; i < VEC; ++i) {
+				const uint32_t at = (c * LANES + lane) * VEC + i;
+				if (at >= width) continue;
+				partial[(uint64_t)blockIdx.x * 2u * width + at] = dscale[c][i];
+				partial[((uint64_t)blockIdx.x * 2u + 1u) * width + at] = dshift[c][i];
+			}
 	}
 }
 
 struct Row {
 	uint32_t lanes, chunks;
 };
-// the fewest lanes that hold a row, one vector each up to 64 lanes, then up to four
+// the fewest lanes that hold a row in one vector each, or in two or four where there are no more lanes to take
 Row row_of(uint32_t width, uint32_t vec) {
-	for (uint32_t lanes = 8; lanes <= 64; lanes *= 2)
-		if (width <= lanes * vec) return {lanes, 1};
-	for (uint32_t lanes : {64u, 256u, 1024u})
-		for (uint32_t chunks : {2u, 4u})
-			if (width <= lanes * chunks * vec) return {lanes, chunks};
+	constexpr Row rows[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {128, 1}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
+	for (const Row& row : rows)
+		if (width <= row.lanes * row.chunks * vec) return row;
 	return {0, 0};
 }
 
@@ -184,10 +260,10 @@ void with_row(Row row, F&& f) {
 	go(integral_constant<uint32_t, 16>{}, integral_constant<uint32_t, 1>{});
 	go(integral_constant<uint32_t, 32>{}, integral_constant<uint32_t, 1>{});
 	go(integral_constant<uint32_t, 64>{}, integral_constant<uint32_t, 1>{});
-	go(integral_constant<uint32_t, 64>{}, integral_constant<uint32_t, 2>{});
-	go(integral_constant<uint32_t, 64>{}, integral_constant<uint32_t, 4>{});
-	go(integral_constant<uint32_t, 256>{}, integral_constant<uint32_t, 2>{});
-	go(integral_constant<uint32_t, 256>{}, integral_constant<uint32_t, 4>{});
+	go(integral_constant<uint32_t, 128>{}, integral_constant<uint32_t, 1>{});
+	go(integral_constant<uint32_t, 256>{}, integral_constant<uint32_t, 1>{});
+	go(integral_constant<uint32_t, 512>{}, integral_constant<uint32_t, 1>{});
+	go(integral_constant<uint32_t, 1024>{}, integral_constant<uint32_t, 1>{});
 	go(integral_constant<uint32_t, 1024>{}, integral_constant<uint32_t, 2>{});
 	go(integral_constant<uint32_t, 1024>{}, integral_constant<uint32_t, 4>{});
 }
@@ -228,7 +304,7 @@ N2_API int n2_layer_norm_forward(n2_stream_t stream, n2_dtype dtype, n2_dtype we
 		using P = decltype(p);
 		with_row(row_of(width, N2Vec<T>::SIZE), [&](auto lanes, auto chunks) {
 			constexpr uint32_t LANES = decltype(lanes)::value, THREADS = threads_of<LANES>(), ROWS = THREADS / LANES;
-			const uint32_t blocks = n2_layer_norm_blocks(n_rows, ROWS, THREADS);
+			const uint32_t blocks = n2_layer_norm_forward_blocks(n_rows, ROWS * rows_at_once<LANES, decltype(chunks)::value, false>(), THREADS);
 			layer_norm_forward_kernel<T, P, LANES, decltype(chunks)::value><<<dim3(blocks), dim3(THREADS), 0, n2_stream(stream)>>>(
 				n_rows, width, epsilon, static_cast<const P*>(d_scale), static_cast<const P*>(d_shift), static_cast<const T*>(d_input), input_stride, static_cast<T*>(d_output),
 				output_stride, d_mean, d_rstd);
@@ -240,9 +316,12 @@ N2_API int n2_layer_norm_forward(n2_stream_t stream, n2_dtype dtype, n2_dtype we
 
 N2_API uint64_t n2_layer_norm_workspace_bytes(n2_dtype dtype, uint32_t n_rows, uint32_t width) {
 	if (!known(dtype) || width < 1 || width > MAX_WIDTH) return 0;
-	const Row row = row_of(width, 16u / n2_dtype_bytes(dtype));
-	const uint32_t threads = row.lanes > 256u ? row.lanes : 256u;
-	return 8ull * width * n2_layer_norm_blocks(n_rows, threads / row.lanes, threads);
+	uint64_t blocks = 0;
+	with_row(row_of(width, 16u / n2_dtype_bytes(dtype)), [&](auto lanes, auto chunks) {
+		constexpr uint32_t LANES = decltype(lanes)::value, THREADS = threads_of<LANES>();
+		blocks = n2_layer_norm_backward_blocks(n_rows, THREADS / LANES * rows_at_once<LANES, decltype(chunks)::value, true>(), THREADS);
+	});
+	return 8ull * width * blocks;
 }
 
 N2_API int n2_layer_norm_backward(n2_stream_t stream, n2_dtype dtype, n2_dtype weights_dtype, uint32_t n_rows, uint32_t width, const void* d_scale, const void* d_input,
@@ -280,7 +359,7 @@ N2_API int n2_layer_norm_backward(n2_stream_t stream, n2_dtype dtype, n2_dtype w
 			using P = decltype(p);
 			with_row(row_of(width, N2Vec<T>::SIZE), [&](auto lanes, auto chunks) {
 				constexpr uint32_t LANES = decltype(lanes)::value, THREADS = threads_of<LANES>(), ROWS = THREADS / LANES;
-				blocks = n2_layer_norm_blocks(n_rows, ROWS, THREADS);
+				blocks = n2_layer_norm_backward_blocks(n_rows, ROWS * rows_at_once<LANES, decltype(chunks)::value, true>(), THREADS);
 				layer_norm_backward_kernel<T, P, LANES, decltype(chunks)::value><<<dim3(blocks), dim3(THREADS), 0, s>>>(
 					n_rows, width, static_cast<const P*>(d_scale), static_cast<const T*>(d_input), input_stride, d_mean, d_rstd, static_cast<const T*>(d_dL_doutput), dL_doutput_stride,
 					static_cast<const T*>(d_dL_dskip), dL_dskip_stride, static_cast<T*>(d_dL_dinput), dL_dinput_stride, weights ? static_cast<float*>(d_workspace) : nullptr);

@@ -2,6 +2,8 @@
 #pragma once
 #include "n2_common.h"
 
+#include <type_traits>
+
 typedef _Float16 n2_f16;
 typedef __bf16 n2_bf16;
 
@@ -34,10 +36,45 @@ __device__ __forceinline__ void n2_store_vec(T* __restrict__ p, const N2Vec<T>& 
 			if (i < valid) p[i] = r.v[i];
 	}
 }
+// The vector at element `at` of a matrix whose last element is before `end`, zero from `valid` on.  Where a row's end leaves part of a vector
+// the rest is read with it as long as the matrix goes on; a lane that reads element by element holds up its whole wave.
+template <typename T>
+__device__ __forceinline__ N2Vec<T> n2_load_row(const T* __restrict__ base, uint64_t at, uint64_t end, uint32_t valid) {
+	if (at + N2Vec<T>::SIZE > end) return n2_load_vec(base + at, valid);
+	N2Vec<T> r;
+	__builtin_memcpy(&r, base + at, 16);
+	if (valid < N2Vec<T>::SIZE) {
+#pragma unroll
+		for (uint32_t i = 0; i < N2Vec<T>::SIZE; ++i) r.v[i] = i < valid ? r.v[i] : (T)0.f;
+	}
+	return r;
+}
 // elements of a row of `width` from place `at` on, at most a vector
 template <typename T>
 __device__ __forceinline__ uint32_t n2_left(uint32_t width, uint32_t at) {
 	return at < width ? min(width - at, N2Vec<T>::SIZE) : 0u;
+}
+
+// Sums over groups of 8, 16, 32 or 64 lanes, in all of them, without LDS: mirrors within the rows of 16 lanes, then whole rows change places.
+template <uint32_t LANES>
+__device__ __forceinline__ float n2_lane_sum(float x) {
+	auto dpp = [](float v, auto control) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(control)::value, 0xf, 0xf, true)); };
+	x += dpp(x, std::integral_constant<int, 0xB1>{});   // quad_perm 1 0 3 2
+	x += dpp(x, std::integral_constant<int, 0x4E>{});   // quad_perm 2 3 0 1
+	x += dpp(x, std::integral_constant<int, 0x141>{});  // row_half_mirror
+	if constexpr (LANES >= 16u) x += dpp(x, std::integral_constant<int, 0x140>{});  // row_mirror
+	auto sum = [](uint32_t a, uint32_t b) { return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b); };
+	if constexpr (LANES >= 32u) {
+		const uint32_t u = __builtin_bit_cast(uint32_t, x);
+		const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+		x = sum(p[0], p[1]);
+	}
+	if constexpr (LANES >= 64u) {
+		const uint32_t u = __builtin_bit_cast(uint32_t, x);
+		const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+		x = sum(p[0], p[1]);
+	}
+	return x;
 }
 
 static inline uint32_t n2_dtype_bytes(uint32_t dtype) { return dtype == N2_DTYPE_F32 ? 4u : 2u; }

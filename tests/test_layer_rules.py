@@ -16,7 +16,8 @@ extern "C" uint64_t plan(uint32_t m, uint32_t n, uint32_t k, uint32_t* out) {
 }
 extern "C" uint32_t xcd_order(uint32_t block, uint32_t blocks) { return n2_xcd_order(block, blocks); }
 extern "C" void tile_order(uint32_t tile, uint32_t tiles_m, uint32_t tiles_n, uint32_t* out) { n2_tile_order(tile, tiles_m, tiles_n, out[0], out[1]); }
-extern "C" uint32_t norm_blocks(uint32_t rows, uint32_t per, uint32_t threads) { return n2_layer_norm_blocks(rows, per, threads); }
+extern "C" uint32_t norm_forward_blocks(uint32_t rows, uint32_t per, uint32_t threads) { return n2_layer_norm_forward_blocks(rows, per, threads); }
+extern "C" uint32_t norm_backward_blocks(uint32_t rows, uint32_t per, uint32_t threads) { return n2_layer_norm_backward_blocks(rows, per, threads); }
 extern "C" uint32_t sum_blocks(uint32_t rows, uint32_t width) { return n2_linear_sum_blocks(rows, width); }
 """
 
@@ -73,8 +74,8 @@ def test_every_tile_comes_once(rules, m, n):
 def test_blocks_of_the_passes_over_rows(rules):
     for rows in (1, 3, 4, 255, 4097, 1 << 20, (1 << 32) - 1):
         for per, threads in ((32, 256), (4, 256), (1, 256), (1, 1024)):
-            blocks = rules.norm_blocks(rows, per, threads)
-            assert 1 <= blocks <= 1024 and (blocks - 1) * per < rows
+            for blocks, most in ((rules.norm_forward_blocks(rows, per, threads), 2048), (rules.norm_backward_blocks(rows, per, threads), 1024)):
+                assert 1 <= blocks <= most and (blocks - 1) * per < rows
         for width in (1, 64, 65, 256, 257, 4096, 65536):
             assert 1 <= rules.sum_blocks(rows, width) <= 1024
-    assert rules.norm_blocks(0, 4, 256) == 0 and rules.sum_blocks(0, 8) == 0
+    assert rules.norm_forward_blocks(0, 4, 256) == rules.norm_backward_blocks(0, 4, 256) == 0 and rules.sum_blocks(0, 8) == 0
