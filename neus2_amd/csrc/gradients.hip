@@ -1,7 +1,7 @@
 // The norm over the gradients of many tensors and their clipping: two launches whatever the number of tensors.
-// The host cuts the tensors into pieces of PIECE values; a launch's workgroups take pieces in turn.  What bounds both launches
-// is memory: the first reads every gradient, the second reads and writes it, from the last pieces to the first, so that what the first
-// launch read last is still in the caches.
+// The host cuts the tensors into pieces, about as many as there are workgroups at a time; a launch's workgroups take pieces in turn.  What
+// bounds both launches is memory: the first reads every gradient, the second reads and writes it, from the last pieces to the first, so that
+// what the first launch read last is still in the caches.
 #include "layer_types.h"
 
 #include <algorithm>
@@ -19,7 +19,9 @@ struct Piece {
 };
 static_assert(sizeof(Piece) == 32, "pieces are read by 16 bytes");
 
-constexpr uint32_t THREADS = 256, PIECE = 8192, MAX_BLOCKS = N2_GRADIENTS_WORKSPACE_BYTES / sizeof(double) / 2;
+constexpr uint32_t THREADS = 256, MAX_BLOCKS = N2_GRADIENTS_WORKSPACE_BYTES / sizeof(double);
+// Bytes to a piece: all pieces at once up to 32 MB, and long enough that a piece's entry in the table costs little beyond.
+constexpr uint64_t PIECE_STEP = THREADS * 16, MOST_STEPS = 16;
 
 // Squares are summed in fp64: those of fp32 and bf16 leave fp32's range long before the values do.
 // (Those of fp16 are exact in fp32, and eight of them lie well inside its range.)
@@ -38,26 +40,38 @@ __device__ __forceinline__ double squares<n2_f16>(const N2Vec<n2_f16>& v) {
 	return (double)s;
 }
 
+// f(vector, place, valid values) for a lane's vectors of a piece, four loads under way at a time
+template <typename T, typename F>
+__device__ __forceinline__ void each_vector(const Piece& p, F&& f) {
+	constexpr uint32_t VEC = N2Vec<T>::SIZE, STEP = THREADS * VEC;
+	const T* in = static_cast<const T*>(p.in);
+	uint32_t at = threadIdx.x * VEC;
+	for (; at + 3u * STEP + VEC <= p.n; at += 4u * STEP) {
+		N2Vec<T> v[4];
+#pragma unroll
+		for (uint32_t i = 0; i < 4u; ++i) __builtin_memcpy(&v[i], in + at + i * STEP, 16);
+#pragma unroll
+		for (uint32_t i = 0; i < 4u; ++i) f(v[i], at + i * STEP, VEC);
+	}
+#pragma unroll
+	for (uint32_t i = 0; i < 4u; ++i, at += STEP)
+		if (at < p.n) f(n2_load_vec(in + at, n2_left<T>(p.n, at)), at, n2_left<T>(p.n, at));
+}
+
 template <typename T>
 __device__ __forceinline__ double piece_squares(const Piece& p) {
-	constexpr uint32_t VEC = N2Vec<T>::SIZE;
 	double s = 0.;
-#pragma unroll 4
-	for (uint32_t at = threadIdx.x * VEC; at < p.n; at += THREADS * VEC) s += squares(n2_load_vec(static_cast<const T*>(p.in) + at, n2_left<T>(p.n, at)));
+	each_vector<T>(p, [&](const N2Vec<T>& v, uint32_t, uint32_t) __attribute__((always_inline)) { s += squares(v); });
 	return s;
 }
 
 template <typename T>
 __device__ __forceinline__ void piece_scale(const Piece& p, float factor) {
-	constexpr uint32_t VEC = N2Vec<T>::SIZE;
-#pragma unroll 4
-	for (uint32_t at = threadIdx.x * VEC; at < p.n; at += THREADS * VEC) {
-		const uint32_t n = n2_left<T>(p.n, at);
-		N2Vec<T> v = n2_load_vec(static_cast<const T*>(p.in) + at, n);
+	each_vector<T>(p, [&](N2Vec<T> v, uint32_t at, uint32_t n) __attribute__((always_inline)) {
 #pragma unroll
-		for (uint32_t i = 0; i < VEC; ++i) v.v[i] = (T)((float)v.v[i] * factor);
+		for (uint32_t i = 0; i < N2Vec<T>::SIZE; ++i) v.v[i] = (T)((float)v.v[i] * factor);
 		n2_store_vec(static_cast<T*>(p.out) + at, v, n);
-	}
+	});
 }
 
 // sum over the workgroup, in all of its lanes
@@ -83,7 +97,11 @@ __global__ void __launch_bounds__(THREADS) gradient_squares_kernel(const Piece* 
 
 __device__ __forceinline__ double norm_of(const double* __restrict__ partial, uint32_t n_partial, double loss_scale) {
 	double s = 0.;
-	for (uint32_t i = threadIdx.x; i < n_partial; i += THREADS) s += partial[i];
+#pragma unroll
+	for (uint32_t k = 0; k < MAX_BLOCKS / THREADS; ++k) {
+		const uint32_t i = k * THREADS + threadIdx.x;
+		s += i < n_partial ? partial[i] : 0.;
+	}
 	return sqrt(block_sum(s)) / loss_scale;
 }
 
@@ -107,7 +125,16 @@ __global__ void __launch_bounds__(THREADS) gradient_clip_kernel(const Piece* __r
 	}
 }
 
-uint64_t pieces_of(uint64_t n) { return n / PIECE + (n % PIECE != 0); }
+// values to a piece of a tensor of this type where all tensors have so many bytes
+uint64_t piece_values(uint64_t all_bytes, uint32_t dtype) {
+	const uint64_t steps = std::min<uint64_t>(std::max<uint64_t>((all_bytes + MAX_BLOCKS * PIECE_STEP - 1) / (MAX_BLOCKS * PIECE_STEP), 1), MOST_STEPS);
+	return steps * PIECE_STEP / n2_dtype_bytes(dtype);
+}
+uint64_t all_bytes_of(uint32_t n_tensors, const n2_gradient_tensor* tensors) {
+	uint64_t bytes = 0;
+	for (uint32_t i = 0; i < n_tensors; ++i) bytes += std::min<uint64_t>(tensors[i].n, 1ull << 44) * n2_dtype_bytes(tensors[i].dtype);
+	return bytes;
+}
 
 }  // namespace
 
@@ -119,7 +146,11 @@ struct n2_gradients {
 N2_API uint64_t n2_gradients_table_bytes(uint32_t n_tensors, const n2_gradient_tensor* tensors) {
 	if (n_tensors > 0 && tensors == nullptr) return 0;
 	uint64_t pieces = 0;
-	for (uint32_t i = 0; i < n_tensors; ++i) pieces += pieces_of(tensors[i].n);
+	const uint64_t all = all_bytes_of(n_tensors, tensors);
+	for (uint32_t i = 0; i < n_tensors; ++i) {
+		const uint64_t values = piece_values(all, tensors[i].dtype);
+		pieces += tensors[i].n / values + (tensors[i].n % values != 0);
+	}
 	return std::max<uint64_t>(pieces, 1) * sizeof(Piece);
 }
 
@@ -131,6 +162,7 @@ N2_API int n2_gradients_create(n2_stream_t stream, uint32_t n_tensors, const n2_
 		struct Range { uintptr_t begin, end; };
 		std::vector<Range> ranges;
 		std::vector<Piece> pieces;
+		const uint64_t all = all_bytes_of(n_tensors, tensors);
 		for (uint32_t i = 0; i < n_tensors; ++i) {
 			const n2_gradient_tensor& t = tensors[i];
 			N2_REQUIRE(t.dtype <= N2_DTYPE_F32, "n2_gradients_create: tensor %u has type %u", i, t.dtype);
@@ -142,8 +174,9 @@ N2_API int n2_gradients_create(n2_stream_t stream, uint32_t n_tensors, const n2_
 			const uintptr_t in = reinterpret_cast<uintptr_t>(t.d_gradients), to = reinterpret_cast<uintptr_t>(t.d_out);
 			ranges.push_back({in, in + t.n * bytes});
 			if (to != in) ranges.push_back({to, to + t.n * bytes});
-			for (uint64_t at = 0; at < t.n; at += PIECE)
-				pieces.push_back({static_cast<const char*>(t.d_gradients) + at * bytes, static_cast<char*>(t.d_out) + at * bytes, (uint32_t)std::min<uint64_t>(PIECE, t.n - at), t.dtype, 0});
+			const uint64_t values = piece_values(all, t.dtype);
+			for (uint64_t at = 0; at < t.n; at += values)
+				pieces.push_back({static_cast<const char*>(t.d_gradients) + at * bytes, static_cast<char*>(t.d_out) + at * bytes, (uint32_t)std::min<uint64_t>(values, t.n - at), t.dtype, 0});
 		}
 		std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
 		for (size_t i = 1; i < ranges.size(); ++i) N2_REQUIRE(ranges[i].begin >= ranges[i - 1].end, "n2_gradients_create: two of the tensors overlap");

@@ -93,7 +93,7 @@ def test_gradients_refuse():
         refused(create(tensors)[0], text)
     refused(create([(A, A, 8, 0)], table=0)[0], "table")
     refused(create([(A, A, 8, 0)], table=W + 8)[0], "table")
-    refused(create([(A, A, 8193, 0)], nbytes=63)[0], "table")
+    refused(create([(A, A, 8193, 0)], nbytes=31)[0], "table")
     rc, h = create([(0, 0, 0, 0)])  # no values: nothing to upload
     assert rc == 0
     L = lib()
