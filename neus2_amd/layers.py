@@ -11,43 +11,56 @@ import torch
 
 from . import capi
 from .capi import GRAD_IGNORE, GRAD_OVERWRITE, N2Error, check
-from .tcnn_api import _address, _stream_address
+from .tcnn_api import _address, _raw_stream, _stream_address
 
 DTYPES = {torch.float16: capi.DTYPE_F16, torch.bfloat16: capi.DTYPE_BF16, torch.float32: capi.DTYPE_F32}
 ACTIVATIONS = {"None": capi.ACTIVATION_NONE, "ReLU": capi.ACTIVATION_RELU, "SiLU": capi.ACTIVATION_SILU, "GELU": capi.ACTIVATION_GELU}
 
 
+# not part of torch's public interface: where a torch does without it, the public call serves (which looks first whether CUDA is there, 0.3 us)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _check_device(t, what):
-    if not t.is_cuda:
+    """The current device's index, which has to be the tensor's."""
+    device = t.get_device()
+    if device < 0:
         raise N2Error(f"{what} must be a CUDA tensor")
-    if t.device.index != torch.cuda.current_device():
-        raise N2Error(f"{what} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if device != _current_device():
+        raise N2Error(f"{what} is on cuda:{device}, the current device is cuda:{_current_device()}")
+    return device
 
 
-def _matrix(t, dtype, rows, width, what):
+def _stream_of(device):
+    return _stream_address() if _raw_stream is None else _raw_stream(device)
+
+
+def _matrix(t, dtype, device, rows, width, what):
     """The row stride of a [rows, width] tensor (rows None: any)."""
-    _check_device(t, what)
     shape = t.shape
-    if t.dtype != dtype or len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows):
+    if t.dtype is not dtype or len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows):
         raise N2Error(f"{what} must be a {dtype} tensor [{'N' if rows is None else rows}, {width}], got {t.dtype} {tuple(shape)}")
-    if shape[0] >= 1 << 31:
-        raise N2Error(f"{what} has {shape[0]} rows, 2^31 - 1 are the most")
-    if t.numel() == 0:
+    if t.get_device() != device:
+        _check_device(t, what)
+    rows = shape[0]
+    if rows >= 1 << 31:
+        raise N2Error(f"{what} has {rows} rows, 2^31 - 1 are the most")
+    if rows == 0:
         return width
     stride, inner = t.stride()
-    if (inner != 1 and width > 1) or (stride < width and shape[0] > 1):
+    if (inner != 1 and width > 1) or (stride < width and rows > 1):
         raise N2Error(f"{what} must have its rows' values side by side and its rows apart, got strides {t.stride()}")
-    return max(stride, width)
+    return stride if stride > width else width
 
 
 def _vector(t, dtype, n, what):
     _check_device(t, what)
-    if t.dtype != dtype or t.shape != (n,) or (not t.is_contiguous()):
+    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
         raise N2Error(f"{what} must be a contiguous {dtype} tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
 
 
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _workspace(nbytes, like):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 class Linear:
@@ -81,6 +94,7 @@ class Linear:
             if t is not None:
                 _vector(t, self.dtype, self.n_params(), "linear params/gradients")
         self._params, self._grads = params, gradients
+        self._at, self._grads_at = self._parts(params), self._parts(gradients)
 
     def _parts(self, t):
         """Addresses of the weights and the bias in a parameter vector."""
@@ -91,52 +105,54 @@ class Linear:
     def _ready(self):
         if self._params is None:
             raise N2Error("linear layer: call set_params first")
-        _check_device(self._params, "linear params")
+        return _check_device(self._params, "linear params")
 
     def forward(self, x, residual=None, want_pre_activation=False, out=None):
         """x [N, in]; residual [N, out] or None.  Returns (y [N, out], z [N, out] or None): z = x W^T + b is what backward of an
         activation takes.  out may be the residual itself."""
-        self._ready()
-        i, o = self.n_input_dims, self.n_output_dims
-        x_stride, n = _matrix(x, self.dtype, None, i, "linear input"), x.shape[0]
-        r_stride = _matrix(residual, self.dtype, n, o, "linear residual") if residual is not None else o
-        y = torch.empty(n, o, dtype=self.dtype, device=x.device) if out is None else out
-        y_stride = o if out is None else _matrix(out, self.dtype, n, o, "linear output")
-        z = torch.empty(n, o, dtype=self.dtype, device=x.device) if want_pre_activation else None
+        device = self._ready()
+        i, o, dtype = self.n_input_dims, self.n_output_dims, self.dtype
+        x_stride, n = _matrix(x, dtype, device, None, i, "linear input"), x.shape[0]
+        r_stride = o if residual is None else _matrix(residual, dtype, device, n, o, "linear residual")
+        y, y_stride = (x.new_empty((n, o)), o) if out is None else (out, _matrix(out, dtype, device, n, o, "linear output"))
+        z = x.new_empty((n, o)) if want_pre_activation else None
         lib = capi.lib()
         nbytes = lib.n2_linear_forward_workspace_bytes(n, i, o)
-        ws = _workspace(nbytes, x.device)
-        w, b = self._parts(self._params)
-        check(lib.n2_linear_forward(_stream_address(), *self._kinds, n, i, o, w, b, x.data_ptr(), x_stride, _address(residual), r_stride, y.data_ptr(), y_stride, _address(z), o,
-                                    _address(ws), nbytes), "n2_linear_forward")
+        ws = _workspace(nbytes, x)
+        w, b = self._at
+        rc = lib.n2_linear_forward(_stream_of(device), *self._kinds, n, i, o, w, b, x.data_ptr(), x_stride, _address(residual), r_stride, y.data_ptr(), y_stride, _address(z), o, _address(ws),
+                                   nbytes)
+        if rc:
+            check(rc, "n2_linear_forward")
         return y, z
 
     def backward(self, x, pre_activation, dL_dy, want_input_grad=True, mode=GRAD_OVERWRITE, out=None):
         """Gradients of the layer's parameters go into the vector of set_params (by mode); returns dL/dx [N, in] or None.
         pre_activation: what forward returned (None without an activation).  The residual's gradient is dL_dy."""
-        self._ready()
-        i, o = self.n_input_dims, self.n_output_dims
-        x_stride, n = _matrix(x, self.dtype, None, i, "linear input"), x.shape[0]
-        dy_stride = _matrix(dL_dy, self.dtype, n, o, "dL_dy")
+        device = self._ready()
+        i, o, dtype = self.n_input_dims, self.n_output_dims, self.dtype
+        x_stride, n = _matrix(x, dtype, device, None, i, "linear input"), x.shape[0]
+        dy_stride = _matrix(dL_dy, dtype, device, n, o, "dL_dy")
         z_stride = o
         if self.activation == "None":
             pre_activation = None
         elif pre_activation is None:
             raise N2Error(f"backward of {self.activation} needs the values before it: forward(want_pre_activation=True)")
         else:
-            z_stride = _matrix(pre_activation, self.dtype, n, o, "pre_activation")
+            z_stride = _matrix(pre_activation, dtype, device, n, o, "pre_activation")
         if mode != GRAD_IGNORE and self._grads is None:
             raise N2Error("linear layer: set_params was given no gradients")
         dx, dx_stride = None, i
         if want_input_grad:
-            dx = torch.empty(n, i, dtype=self.dtype, device=x.device) if out is None else out
-            dx_stride = i if out is None else _matrix(out, self.dtype, n, i, "dL_dx")
+            dx, dx_stride = (x.new_empty((n, i)), i) if out is None else (out, _matrix(out, dtype, device, n, i, "dL_dx"))
         lib = capi.lib()
         nbytes = lib.n2_linear_backward_workspace_bytes(n, i, o)
-        ws = _workspace(nbytes, x.device)
-        dw, db = self._parts(self._grads)
-        check(lib.n2_linear_backward(_stream_address(), *self._kinds, n, i, o, self._params.data_ptr(), x.data_ptr(), x_stride, _address(pre_activation), z_stride, dL_dy.data_ptr(),
-                                     dy_stride, _address(dx), dx_stride, dw, db, mode, _address(ws), nbytes), "n2_linear_backward")
+        ws = _workspace(nbytes, x)
+        dw, db = self._grads_at
+        rc = lib.n2_linear_backward(_stream_of(device), *self._kinds, n, i, o, self._at[0], x.data_ptr(), x_stride, _address(pre_activation), z_stride, dL_dy.data_ptr(), dy_stride, _address(dx),
+                                    dx_stride, dw, db, mode, _address(ws), nbytes)
+        if rc:
+            check(rc, "n2_linear_backward")
         return dx
 
 
@@ -170,37 +186,39 @@ class LayerNorm:
             if t is not None:
                 _vector(t, self.param_dtype, self.n_params(), "layer norm params/gradients")
         self._params, self._grads = params, gradients
+        self._at, self._grads_at = self._parts(params), self._parts(gradients)
 
     def _ready(self):
         if self._params is None:
             raise N2Error("layer norm: call set_params first")
-        _check_device(self._params, "layer norm params")
+        return _check_device(self._params, "layer norm params")
 
     def _parts(self, t):
         return (None, None) if t is None else (t.data_ptr(), t.data_ptr() + t.element_size() * self.n_dims)
 
     def forward(self, x, want_ctx=False, out=None):
         """Returns (y, ctx): ctx = (mean, rstd), fp32 [N] each, is what backward takes (None unless asked for)."""
-        self._ready()
-        w = self.n_dims
-        x_stride, n = _matrix(x, self.dtype, None, w, "layer norm input"), x.shape[0]
-        y = torch.empty(n, w, dtype=self.dtype, device=x.device) if out is None else out
-        y_stride = w if out is None else _matrix(out, self.dtype, n, w, "layer norm output")
-        ctx = (torch.empty(n, dtype=torch.float32, device=x.device), torch.empty(n, dtype=torch.float32, device=x.device)) if want_ctx else None
-        mean, rstd = ctx if want_ctx else (None, None)
-        check(capi.lib().n2_layer_norm_forward(_stream_address(), *self._kinds, n, w, self.epsilon, *self._parts(self._params), x.data_ptr(), x_stride, y.data_ptr(), y_stride,
-                                               _address(mean), _address(rstd)), "n2_layer_norm_forward")
+        device = self._ready()
+        w, dtype = self.n_dims, self.dtype
+        x_stride, n = _matrix(x, dtype, device, None, w, "layer norm input"), x.shape[0]
+        y, y_stride = (x.new_empty((n, w)), w) if out is None else (out, _matrix(out, dtype, device, n, w, "layer norm output"))
+        mean = rstd = ctx = None
+        if want_ctx:
+            ctx = mean, rstd = x.new_empty(n, dtype=torch.float32), x.new_empty(n, dtype=torch.float32)
+        rc = capi.lib().n2_layer_norm_forward(_stream_of(device), *self._kinds, n, w, self.epsilon, *self._at, x.data_ptr(), x_stride, y.data_ptr(), y_stride, _address(mean), _address(rstd))
+        if rc:
+            check(rc, "n2_layer_norm_forward")
         return y, ctx
 
     def backward(self, ctx, x, dL_dy, dL_dskip=None, want_input_grad=True, mode=GRAD_OVERWRITE, out=None):
         """dL_dskip (or None): a gradient of x that is added to dL/dx, as a skip connection past the norm has it; out may be that tensor."""
-        self._ready()
+        device = self._ready()
         if ctx is None:
             raise N2Error("layer norm: backward needs the ctx of forward(want_ctx=True)")
-        w = self.n_dims
-        x_stride, n = _matrix(x, self.dtype, None, w, "layer norm input"), x.shape[0]
-        dy_stride = _matrix(dL_dy, self.dtype, n, w, "dL_dy")
-        skip_stride = w if dL_dskip is None else _matrix(dL_dskip, self.dtype, n, w, "dL_dskip")
+        w, dtype = self.n_dims, self.dtype
+        x_stride, n = _matrix(x, dtype, device, None, w, "layer norm input"), x.shape[0]
+        dy_stride = _matrix(dL_dy, dtype, device, n, w, "dL_dy")
+        skip_stride = w if dL_dskip is None else _matrix(dL_dskip, dtype, device, n, w, "dL_dskip")
         mean, rstd = ctx
         _vector(mean, torch.float32, n, "mean")
         _vector(rstd, torch.float32, n, "rstd")
@@ -210,14 +228,14 @@ class LayerNorm:
             raise N2Error("layer norm: dL_dskip without dL/dx")
         dx, dx_stride = None, w
         if want_input_grad:
-            dx = torch.empty(n, w, dtype=self.dtype, device=x.device) if out is None else out
-            dx_stride = w if out is None else _matrix(out, self.dtype, n, w, "dL_dx")
+            dx, dx_stride = (x.new_empty((n, w)), w) if out is None else (out, _matrix(out, dtype, device, n, w, "dL_dx"))
         lib = capi.lib()
         nbytes = lib.n2_layer_norm_workspace_bytes(self._kinds[0], n, w) if mode != GRAD_IGNORE else 0
-        ws = _workspace(nbytes, x.device)
-        check(lib.n2_layer_norm_backward(_stream_address(), *self._kinds, n, w, self._params.data_ptr(), x.data_ptr(), x_stride, mean.data_ptr(), rstd.data_ptr(), dL_dy.data_ptr(),
-                                         dy_stride, _address(dL_dskip), skip_stride, _address(dx), dx_stride, *self._parts(self._grads), mode, _address(ws), nbytes),
-              "n2_layer_norm_backward")
+        ws = _workspace(nbytes, x)
+        rc = lib.n2_layer_norm_backward(_stream_of(device), *self._kinds, n, w, self._at[0], x.data_ptr(), x_stride, mean.data_ptr(), rstd.data_ptr(), dL_dy.data_ptr(), dy_stride,
+                                        _address(dL_dskip), skip_stride, _address(dx), dx_stride, *self._grads_at, mode, _address(ws), nbytes)
+        if rc:
+            check(rc, "n2_layer_norm_backward")
         return dx
 
 
@@ -243,9 +261,8 @@ class GradientClip:
             tensors[i] = capi.GradientTensor(g.data_ptr(), o.data_ptr(), g.numel(), DTYPES[g.dtype])
         L = capi.lib()
         nbytes = L.n2_gradients_table_bytes(len(gradients), tensors)
-        self._device = gradients[0].device if gradients else torch.device("cuda", torch.cuda.current_device())
         self._keep = (gradients, out)
-        self._table = torch.empty(nbytes, dtype=torch.uint8, device=self._device)
+        self._table = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
         self._h = C.c_void_p()
         check(L.n2_gradients_create(_stream_address(), len(gradients), tensors, self._table.data_ptr(), nbytes, C.byref(self._h)), "n2_gradients_create")
 
@@ -258,18 +275,19 @@ class GradientClip:
             pass
 
     def _buffers(self):
-        _check_device(self._table, "the gradients' table")
-        return torch.empty((), dtype=torch.float32, device=self._device), torch.empty(capi.GRADIENTS_WORKSPACE_BYTES, dtype=torch.uint8, device=self._device)
+        table = self._table
+        device = _check_device(table, "the gradients' table")
+        return device, table.new_empty((), dtype=torch.float32), table.new_empty(capi.GRADIENTS_WORKSPACE_BYTES)
 
     def norm(self, loss_scale=1.0):
         """sqrt(sum of squares) / loss_scale as a one-element device tensor (no host synchronisation)."""
-        norm, ws = self._buffers()
-        check(capi.lib().n2_gradients_norm(self._h, _stream_address(), loss_scale, norm.data_ptr(), ws.data_ptr(), ws.numel()), "n2_gradients_norm")
+        device, norm, ws = self._buffers()
+        check(capi.lib().n2_gradients_norm(self._h, _stream_of(device), loss_scale, norm.data_ptr(), ws.data_ptr(), capi.GRADIENTS_WORKSPACE_BYTES), "n2_gradients_norm")
         return norm
 
     def clip(self, max_norm, loss_scale=1.0):
         """Multiplies the gradients by min(1, max_norm / (norm + 1e-6)); they keep their loss scale (Adam.step's, whose gradients
         are loss_scale times the loss's).  Returns the norm before, as norm() does."""
-        norm, ws = self._buffers()
-        check(capi.lib().n2_gradients_clip(self._h, _stream_address(), max_norm, loss_scale, norm.data_ptr(), ws.data_ptr(), ws.numel()), "n2_gradients_clip")
+        device, norm, ws = self._buffers()
+        check(capi.lib().n2_gradients_clip(self._h, _stream_of(device), max_norm, loss_scale, norm.data_ptr(), ws.data_ptr(), capi.GRADIENTS_WORKSPACE_BYTES), "n2_gradients_clip")
         return norm
