@@ -368,6 +368,5 @@ N2_API int n2_layer_norm_backward(n2_stream_t stream, n2_dtype dtype, n2_dtype w
 		N2_LAUNCH_CHECK();
 	}
 	if (!weights) return N2_OK;
-	const N2ColumnOutput scale_out = {d_dL_dscale, 0, width, (uint32_t)weights_dtype}, shift_out = {d_dL_dshift, width, width, (uint32_t)weights_dtype};
-	return n2_column_sums<2>(s, static_cast<const float*>(d_workspace), blocks, 2u * width, scale_out, shift_out, mode == N2_GRAD_ACCUMULATE ? 1 : 0);
+	return n2_column_sums(s, static_cast<const float*>(d_workspace), blocks, width, d_dL_dscale, d_dL_dshift, weights_dtype, mode == N2_GRAD_ACCUMULATE ? 1 : 0);
 }

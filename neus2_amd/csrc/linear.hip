@@ -121,15 +121,16 @@ struct Fragments {
 // -------------------------------------------------------------------------------------------------------------------------------------
 // the product
 // -------------------------------------------------------------------------------------------------------------------------------------
-enum Epilogue { LAYER, STORE, GRADIENT, PARTIAL };
+enum Epilogue { LAYER, STORE, GRADIENT };
 
 struct Product {
 	Operand a, b;
 	uint32_t m, n, k;
 	uint32_t extent_a, extent_b;  // indices that may be read (of an operand contiguous in them a multiple of eight)
-	uint32_t tiles_m, tiles_n, k_per_split;
-	void* c;              // T [m][n], PARTIAL: fp32 [splits][m][n]
+	uint32_t tiles_m, tiles_n, splits, k_per_split;
+	void* c;         // T [m][n]
 	uint64_t ldc;
+	float* partial;  // or null: the sums of the splits, [splits][m][n], instead of C
 	// LAYER
 	const void* bias;
 	const void* residual;
@@ -159,8 +160,8 @@ __device__ __forceinline__ void finish(const Product& q, uint32_t m, uint32_t n,
 		for (uint32_t i = 0; i < N; ++i) t.v[i] = (std::remove_pointer_t<decltype(p)>)v[i];
 		__builtin_memcpy(p, &t, sizeof(t));
 	};
-	if constexpr (EPI == PARTIAL) {
-		store(static_cast<float*>(q.c) + ((uint64_t)split * q.m + m) * q.n + n);
+	if (q.partial != nullptr) {
+		store(q.partial + ((uint64_t)split * q.m + m) * q.n + n);
 	} else {
 		T* c = static_cast<T*>(q.c) + (uint64_t)m * q.ldc + n;
 		if constexpr (EPI == LAYER) {
@@ -215,10 +216,9 @@ __device__ __forceinline__ void finish_all(const Product& q, uint32_t m0, uint32
 // BM x BN of C to a workgroup, WM x WN waves.  The matrix instruction's rows are n and its columns m, so that a lane's four values stand side
 // by side in a row of C; where B is contiguous in k its rows are dealt to the instructions so that all of a lane's values do.
 template <typename T, bool A_KC, bool B_KC, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, int EPI>
-__global__ void __launch_bounds__(WM* WN * 64) product_kernel(Product q) {
+__device__ __forceinline__ void product(const Product& q, uint32_t block, uint4* __restrict__ tile_a, uint4* __restrict__ tile_b) {
 	constexpr uint32_t THREADS = WM * WN * 64u, S = BM / WM / 16u, U = BN / WN / 16u, RUN = B_KC ? 8u : 4u;
-	__shared__ uint4 tile_a[BM * BK / 8u], tile_b[BN * BK / 8u];
-	const uint32_t tile = blockIdx.x % (q.tiles_m * q.tiles_n), split = blockIdx.x / (q.tiles_m * q.tiles_n);
+	const uint32_t tile = block % (q.tiles_m * q.tiles_n), split = block / (q.tiles_m * q.tiles_n);
 	const uint32_t m0 = tile / q.tiles_n * BM, n0 = tile % q.tiles_n * BN;
 	const uint32_t wave = threadIdx.x / 64u, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
 	const uint32_t k_begin = split * q.k_per_split, k_end = min(q.k, k_begin + q.k_per_split);
@@ -315,10 +315,9 @@ __device__ __forceinline__ void product_stage(const uint4* __restrict__ ta, cons
 
 // Two stages in LDS, 128 KiB, and eight waves of 128 x 64: a CU's LDS reads 96 of its 128 bytes a clock under full matrix cores.
 template <typename T, bool A_KC, bool B_KC, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, int EPI>
-__global__ void __launch_bounds__(WM* WN * 64) product_async_kernel(Product q) {
+__device__ __forceinline__ void product_async(const Product& q, uint32_t block, uint32_t blocks, uint4* tile_a0, uint4* tile_a1, uint4* tile_b0, uint4* tile_b1) {
 	constexpr uint32_t THREADS = WM * WN * 64u, S = BM / WM / 16u, U = BN / WN / 16u, RUN = B_KC ? 8u : 4u;
-	__shared__ uint4 tile_a0[BM * BK / 8u], tile_a1[BM * BK / 8u], tile_b0[BN * BK / 8u], tile_b1[BN * BK / 8u];
-	const uint32_t tiles = q.tiles_m * q.tiles_n, work = n2_xcd_order(blockIdx.x, gridDim.x), split = work / tiles;
+	const uint32_t tiles = q.tiles_m * q.tiles_n, work = n2_xcd_order(block, blocks), split = work / tiles;
 	uint32_t tm, tn;
 	n2_tile_order(work - split * tiles, q.tiles_m, q.tiles_n, tm, tn);
 	const uint32_t m0 = tm * BM, n0 = tn * BN;
@@ -355,11 +354,33 @@ __global__ void __launch_bounds__(WM* WN * 64) product_async_kernel(Product q) {
 	finish_all<T, EPI, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a0));
 }
 
-// The sums of the parts that k was dealt out to, [splits][m][n], finished: a lane takes four columns of a row.
+template <typename T, bool ASYNC, bool A_KC, bool B_KC, uint32_t B, uint32_t WM, uint32_t WN, int EPI>
+__global__ void __launch_bounds__(WM* WN * 64) product_kernel(Product q) {
+	__shared__ uint4 a0[B * BK / 8u], b0[B * BK / 8u], a1[ASYNC ? B * BK / 8u : 1u], b1[ASYNC ? B * BK / 8u : 1u];
+	if constexpr (ASYNC) product_async<T, A_KC, B_KC, B, B, WM, WN, EPI>(q, blockIdx.x, gridDim.x, a0, a1, b0, b1);
+	else product<T, A_KC, B_KC, B, B, WM, WN, EPI>(q, blockIdx.x, a0, b0);
+}
+
+// Both products of a backward pass in one launch, where they are small: the first blocks_x workgroups are dx's.
+template <typename T, bool ASYNC>
+__global__ void __launch_bounds__(256) product_pair_kernel(Product x, Product w, uint32_t blocks_x) {
+	__shared__ uint4 a0[64u * BK / 8u], b0[64u * BK / 8u], a1[ASYNC ? 64u * BK / 8u : 1u], b1[ASYNC ? 64u * BK / 8u : 1u];
+	if (blockIdx.x < blocks_x) {
+		if constexpr (ASYNC) product_async<T, true, false, 64, 64, 2, 2, STORE>(x, blockIdx.x, blocks_x, a0, a1, b0, b1);
+		else product<T, true, false, 64, 64, 2, 2, STORE>(x, blockIdx.x, a0, b0);
+	} else {
+		if constexpr (ASYNC) product_async<T, false, false, 64, 64, 2, 2, GRADIENT>(w, blockIdx.x - blocks_x, gridDim.x - blocks_x, a0, a1, b0, b1);
+		else product<T, false, false, 64, 64, 2, 2, GRADIENT>(w, blockIdx.x - blocks_x, a0, b0);
+	}
+}
+
+// The sums of the parts that k was dealt out to, finished: a lane takes four columns of a row.
 template <typename T, int EPI>
-__global__ void __launch_bounds__(256) join_kernel(Product q, const float* __restrict__ partial, uint32_t splits) {
+__device__ __forceinline__ void join(Product q, uint32_t block) {
+	const float* partial = q.partial;
+	q.partial = nullptr;
 	const uint32_t quads = n2_ceil_div(q.n, 4u);
-	const uint64_t at = (uint64_t)blockIdx.x * 256u + threadIdx.x, row = at / quads;
+	const uint64_t at = (uint64_t)block * 256u + threadIdx.x, row = at / quads;
 	if (row >= q.m) return;
 	const uint32_t m = (uint32_t)row, n = (uint32_t)(at - row * quads) * 4u, valid = min(q.n - n, 4u);
 	float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -367,7 +388,7 @@ __global__ void __launch_bounds__(256) join_kernel(Product q, const float* __res
 	const uint64_t pitch = (uint64_t)q.m * q.n;
 	if (valid == 4u) {
 #pragma unroll 8
-		for (uint32_t i = 0; i < splits; ++i) {
+		for (uint32_t i = 0; i < q.splits; ++i) {
 			float t[4];
 			__builtin_memcpy(t, p + i * pitch, 16);
 			v[0] += t[0], v[1] += t[1], v[2] += t[2], v[3] += t[3];
@@ -376,10 +397,24 @@ __global__ void __launch_bounds__(256) join_kernel(Product q, const float* __res
 	} else {
 		for (uint32_t j = 0; j < valid; ++j) {
 			float w[1] = {0.f};
-			for (uint32_t i = 0; i < splits; ++i) w[0] += p[i * pitch + j];
+			for (uint32_t i = 0; i < q.splits; ++i) w[0] += p[i * pitch + j];
 			finish<T, EPI>(q, m, n + j, 0u, w);
 		}
 	}
+}
+uint32_t join_blocks(const Product& q) { return q.partial != nullptr ? n2_ceil_div((uint64_t)q.m * n2_ceil_div(q.n, 4u), 256u) : 0u; }
+
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(Product q) { join<T, LAYER>(q, blockIdx.x); }
+
+// What is left of a backward pass: dx's and dW's splits, and the bias's gradient from the column sums of sum_rows workgroups.
+template <typename T>
+__global__ void __launch_bounds__(256) join_backward_kernel(Product x, uint32_t blocks_x, Product w, uint32_t blocks_w, const float* __restrict__ sums, uint32_t sum_rows, uint32_t columns,
+                                                            T* __restrict__ db, int accumulate) {
+	const uint32_t block = blockIdx.x;
+	if (block < blocks_x) join<T, STORE>(x, block);
+	else if (block - blocks_x < blocks_w) join<T, GRADIENT>(w, block - blocks_x);
+	else n2_column_sums_block<16, 1, 16>(sums, sum_rows, columns, block - blocks_x - blocks_w, [&](uint32_t column, float sum) { n2_store_sum(db + column, sum, accumulate); });
 }
 
 // -------------------------------------------------------------------------------------------------------------------------------------
@@ -432,38 +467,31 @@ bool async_operand(const Operand& o, bool kc, uint32_t extent, uint32_t k) {
 	return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % 8 == 0 && o.ld < (1u << 22) && (o.padded || (kc ? k : extent) % 8 == 0);
 }
 
-// C by the plan; partial: n2_linear_partial_bytes of it
-template <typename T, bool A_KC, bool B_KC, int EPI>
-int launch_product(hipStream_t s, Product q, const N2LinearPlan& plan, float* partial) {
-	q.k_per_split = plan.k_per_split;
+template <bool A_KC, bool B_KC>
+bool async_product(const Product& q) { return async_operand(q.a, A_KC, q.extent_a, q.k) && async_operand(q.b, B_KC, q.extent_b, q.k); }
+
+// how the product is cut, with `partial` for the sums of splits
+void plan_product(Product& q, const N2LinearPlan& plan, float* partial) {
 	if (q.extent_a == 0) q.extent_a = q.m;
 	if (q.extent_b == 0) q.extent_b = q.n;
 	q.tiles_m = n2_ceil_div(q.m, plan.tile), q.tiles_n = n2_ceil_div(q.n, plan.tile);
-	const uint64_t blocks = (uint64_t)q.tiles_m * q.tiles_n * plan.splits;
-	N2_REQUIRE(blocks <= 0xFFFFFFFFull / 512u, "n2_linear: %u x %u values take %llu workgroups", q.m, q.n, (unsigned long long)blocks);
-	auto launch = [&](auto epi, const Product& p) {
-		constexpr int E = decltype(epi)::value;
-		const dim3 grid((uint32_t)blocks);
-		if (async_operand(q.a, A_KC, q.extent_a, q.k) && async_operand(q.b, B_KC, q.extent_b, q.k)) {
-			if (plan.tile == 256) product_async_kernel<T, A_KC, B_KC, 256, 256, 2, 4, E><<<grid, dim3(512), 0, s>>>(p);
-			else if (plan.tile == 128) product_async_kernel<T, A_KC, B_KC, 128, 128, 2, 2, E><<<grid, dim3(256), 0, s>>>(p);
-			else product_async_kernel<T, A_KC, B_KC, 64, 64, 2, 2, E><<<grid, dim3(256), 0, s>>>(p);
-		} else {
-			if (plan.tile == 256) product_kernel<T, A_KC, B_KC, 256, 256, 2, 4, E><<<grid, dim3(512), 0, s>>>(p);
-			else if (plan.tile == 128) product_kernel<T, A_KC, B_KC, 128, 128, 2, 2, E><<<grid, dim3(256), 0, s>>>(p);
-			else product_kernel<T, A_KC, B_KC, 64, 64, 2, 2, E><<<grid, dim3(256), 0, s>>>(p);
-		}
+	q.splits = plan.splits, q.k_per_split = plan.k_per_split;
+	q.partial = plan.splits > 1 ? partial : nullptr;
+}
+uint64_t blocks_of(const Product& q) { return (uint64_t)q.tiles_m * q.tiles_n * q.splits; }
+
+template <typename T, bool A_KC, bool B_KC, int EPI>
+int launch_product(hipStream_t s, const Product& q, uint32_t tile) {
+	N2_REQUIRE(blocks_of(q) <= 0xFFFFFFFFull / 512u, "n2_linear: %u x %u values take %llu workgroups", q.m, q.n, (unsigned long long)blocks_of(q));
+	const dim3 grid((uint32_t)blocks_of(q));
+	auto launch = [&](auto async) {
+		constexpr bool ASYNC = decltype(async)::value;
+		if (tile == 256) product_kernel<T, ASYNC, A_KC, B_KC, 256, 2, 4, EPI><<<grid, dim3(512), 0, s>>>(q);
+		else if (tile == 128) product_kernel<T, ASYNC, A_KC, B_KC, 128, 2, 2, EPI><<<grid, dim3(256), 0, s>>>(q);
+		else product_kernel<T, ASYNC, A_KC, B_KC, 64, 2, 2, EPI><<<grid, dim3(256), 0, s>>>(q);
 	};
-	if (plan.splits <= 1) {
-		launch(std::integral_constant<int, EPI>{}, q);
-	} else {
-		Product part = q;
-		part.c = partial;
-		launch(std::integral_constant<int, PARTIAL>{}, part);
-		N2_LAUNCH_CHECK();
-		const uint64_t lanes = (uint64_t)q.m * n2_ceil_div(q.n, 4u);
-		join_kernel<T, EPI><<<dim3((uint32_t)((lanes + 255u) / 256u)), dim3(256), 0, s>>>(q, partial, plan.splits);
-	}
+	if (async_product<A_KC, B_KC>(q)) launch(std::true_type{});
+	else launch(std::false_type{});
 	N2_LAUNCH_CHECK();
 	return N2_OK;
 }
@@ -477,7 +505,7 @@ constexpr uint32_t MAX_WIDTH = 65536;
 
 // what a backward pass keeps in its workspace, in this order
 struct BackwardPlan {
-	uint64_t ld_dz, dz_bytes, sums_bytes, partial_bytes;
+	uint64_t ld_dz, dz_bytes, sums_bytes, partial_bytes, input_partial;
 	uint32_t sum_blocks;
 	N2LinearPlan input, weights;
 };
@@ -489,8 +517,8 @@ BackwardPlan backward_plan(uint32_t n_rows, uint32_t in_width, uint32_t out_widt
 	p.sums_bytes = ((uint64_t)p.sum_blocks * out_width * 4u + 15u) / 16u * 16u;
 	p.input = n2_linear_plan(n_rows, in_width, out_width);
 	p.weights = n2_linear_plan(out_width, in_width, n_rows);
-	const uint64_t a = n2_linear_partial_bytes(p.input, n_rows, in_width), b = n2_linear_partial_bytes(p.weights, out_width, in_width);
-	p.partial_bytes = a > b ? a : b;
+	p.input_partial = n2_linear_partial_bytes(p.input, n_rows, in_width) / 4u;
+	p.partial_bytes = p.input_partial * 4u + n2_linear_partial_bytes(p.weights, out_width, in_width);
 	return p;
 }
 
@@ -531,7 +559,17 @@ N2_API int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation a
 	q.m = n_rows, q.n = out_width, q.k = in_width;
 	q.c = d_output, q.ldc = output_stride;
 	q.bias = d_bias, q.residual = d_residual, q.ldr = residual_stride, q.pre = d_pre_activation, q.ldp = pre_stride, q.activation = activation;
-	return with_type(dtype, [&](auto t) { return launch_product<decltype(t), true, true, LAYER>(n2_stream(stream), q, n2_linear_plan(n_rows, out_width, in_width), static_cast<float*>(d_workspace)); });
+	const N2LinearPlan plan = n2_linear_plan(n_rows, out_width, in_width);
+	plan_product(q, plan, static_cast<float*>(d_workspace));
+	return with_type(dtype, [&](auto t) -> int {
+		using T = decltype(t);
+		if (const int rc = launch_product<T, true, true, LAYER>(n2_stream(stream), q, plan.tile)) return rc;
+		if (q.partial != nullptr) {
+			join_kernel<T><<<dim3(join_blocks(q)), dim3(256), 0, n2_stream(stream)>>>(q);
+			N2_LAUNCH_CHECK();
+		}
+		return N2_OK;
+	});
 }
 
 N2_API uint64_t n2_linear_backward_workspace_bytes(uint32_t n_rows, uint32_t in_width, uint32_t out_width) {
@@ -588,24 +626,37 @@ N2_API int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation 
 			else launch(std::integral_constant<uint32_t, 64>{});
 			N2_LAUNCH_CHECK();
 		}
-		if (d_dL_dinput != nullptr && n_rows > 0) {
-			Product q = {};
-			q.a = dz, q.b = {d_weights, in_width, false};
-			q.m = n_rows, q.n = in_width, q.k = out_width;
-			q.c = d_dL_dinput, q.ldc = dL_dinput_stride;
-			if (const int rc = launch_product<T, true, false, STORE>(s, q, p.input, partial)) return rc;
+		Product x = {}, w = {};
+		const bool has_x = d_dL_dinput != nullptr && n_rows > 0;
+		if (has_x) {
+			x.a = dz, x.b = {d_weights, in_width, false};
+			x.m = n_rows, x.n = in_width, x.k = out_width;
+			x.c = d_dL_dinput, x.ldc = dL_dinput_stride;
+			plan_product(x, p.input, partial);
 		}
 		if (dw != nullptr) {
-			Product q = {};
-			q.a = dz, q.b = {d_input, input_stride, false};
-			q.m = out_width, q.n = in_width, q.k = n_rows;
-			if (dz.padded) q.extent_a = (uint32_t)p.ld_dz;
-			q.c = dw, q.ldc = in_width, q.accumulate = accumulate;
-			if (const int rc = launch_product<T, false, false, GRADIENT>(s, q, p.weights, partial)) return rc;
+			w.a = dz, w.b = {d_input, input_stride, false};
+			w.m = out_width, w.n = in_width, w.k = n_rows;
+			if (dz.padded) w.extent_a = (uint32_t)p.ld_dz;
+			w.c = dw, w.ldc = in_width, w.accumulate = accumulate;
+			plan_product(w, p.weights, partial + p.input_partial);
 		}
-		if (db != nullptr) {
-			const N2ColumnOutput out = {db, 0, out_width, (uint32_t)dtype};
-			if (const int rc = n2_column_sums<1>(s, sums, n_rows > 0 ? p.sum_blocks : 0u, out_width, out, out, accumulate)) return rc;
+		const bool async = async_product<true, false>(x);
+		if (has_x && dw != nullptr && p.input.tile == 64 && p.weights.tile == 64 && async == async_product<false, false>(w) && blocks_of(x) + blocks_of(w) <= 0xFFFFFFFFull / 512u) {
+			const dim3 grid((uint32_t)(blocks_of(x) + blocks_of(w)));
+			if (async) product_pair_kernel<T, true><<<grid, dim3(256), 0, s>>>(x, w, (uint32_t)blocks_of(x));
+			else product_pair_kernel<T, false><<<grid, dim3(256), 0, s>>>(x, w, (uint32_t)blocks_of(x));
+			N2_LAUNCH_CHECK();
+		} else {
+			if (has_x)
+				if (const int rc = launch_product<T, true, false, STORE>(s, x, p.input.tile)) return rc;
+			if (dw != nullptr)
+				if (const int rc = launch_product<T, false, false, GRADIENT>(s, w, p.weights.tile)) return rc;
+		}
+		const uint32_t blocks_x = join_blocks(x), blocks_w = join_blocks(w), blocks_b = db != nullptr ? n2_ceil_div(out_width, 16u) : 0u;
+		if (blocks_x + blocks_w + blocks_b > 0) {
+			join_backward_kernel<T><<<dim3(blocks_x + blocks_w + blocks_b), dim3(256), 0, s>>>(x, blocks_x, w, blocks_w, sums, n_rows > 0 ? p.sum_blocks : 0u, out_width, static_cast<T*>(db), accumulate);
+			N2_LAUNCH_CHECK();
 		}
 		return N2_OK;
 	});
