@@ -21,19 +21,31 @@ __device__ __forceinline__ f32x4 mfma(n2_bf16, s16x8 a, s16x8 b, f32x4 c) {
 	return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// exp2 and the reciprocal are the hardware's, within a step of fp32; what the exponent's rounding adds to exp(-|z|) is below 2^-24 |z| of it.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+// 1 + erf(z / sqrt(2)) by the rational approximation 7.1.26 of Abramowitz and Stegun's handbook, within 1.5e-7, given exp(-z^2 / 2).  (The
+// mathematical library's erff took 50 us of 174 for 16384 x 2048 values, three times the product's own epilogue.)
+__device__ __forceinline__ float one_plus_erf(float z, float gauss) {
+	const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.f));
+	const float tail = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * gauss;
+	return z < 0.f ? tail : 2.f - tail;
+}
 __device__ __forceinline__ float activation(float z, int kind) {
 	if (kind == N2_ACTIVATION_RELU) return z > 0.f ? z : 0.f;
-	if (kind == N2_ACTIVATION_SILU) return z / (1.f + expf(-z));
-	if (kind == N2_ACTIVATION_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+	if (kind == N2_ACTIVATION_SILU) return z * __builtin_amdgcn_rcpf(1.f + fast_exp(-z));
+	if (kind == N2_ACTIVATION_GELU) return 0.5f * z * one_plus_erf(z, fast_exp(-0.5f * z * z));
 	return z;
 }
 __device__ __forceinline__ float activation_slope(float z, int kind) {
 	if (kind == N2_ACTIVATION_RELU) return z > 0.f ? 1.f : 0.f;
 	if (kind == N2_ACTIVATION_SILU) {
-		const float s = 1.f / (1.f + expf(-z));
-		return s * (1.f + z * (1.f - s));
+		const float s = __builtin_amdgcn_rcpf(1.f + fast_exp(-z));
+		return s * fmaf(z, 1.f - s, 1.f);
 	}
-	if (kind == N2_ACTIVATION_GELU) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+	if (kind == N2_ACTIVATION_GELU) {
+		const float gauss = fast_exp(-0.5f * z * z);
+		return fmaf(z * gauss, 0.39894228040143268f, 0.5f * one_plus_erf(z, gauss));
+	}
 	return 1.f;
 }
 
@@ -122,6 +134,8 @@ struct Fragments {
 // the product
 // -------------------------------------------------------------------------------------------------------------------------------------
 enum Epilogue { LAYER, STORE, GRADIENT };
+// C, or the sums of one split of k: known where the kernel is built (a test in the epilogue costs large products 2 %), or by Product::partial
+enum Output { WHOLE, SPLIT, EITHER };
 
 struct Product {
 	Operand a, b;
@@ -146,7 +160,7 @@ struct Run {
 	T v[N];
 };
 // N consecutive values of row m from column n on, all of them inside
-template <typename T, int EPI, uint32_t N>
+template <typename T, int EPI, int OUT, uint32_t N>
 __device__ __forceinline__ void finish(const Product& q, uint32_t m, uint32_t n, uint32_t split, float (&v)[N]) {
 	auto add = [&](const T* p) __attribute__((always_inline)) {
 		Run<T, N> t;
@@ -160,7 +174,7 @@ __device__ __forceinline__ void finish(const Product& q, uint32_t m, uint32_t n,
 		for (uint32_t i = 0; i < N; ++i) t.v[i] = (std::remove_pointer_t<decltype(p)>)v[i];
 		__builtin_memcpy(p, &t, sizeof(t));
 	};
-	if (q.partial != nullptr) {
+	if (OUT == SPLIT || (OUT == EITHER && q.partial != nullptr)) {
 		store(q.partial + ((uint64_t)split * q.m + m) * q.n + n);
 	} else {
 		T* c = static_cast<T*>(q.c) + (uint64_t)m * q.ldc + n;
@@ -180,7 +194,7 @@ __device__ __forceinline__ void finish(const Product& q, uint32_t m, uint32_t n,
 
 // What a wave has of C, from (m0, n0) on.  Inside C a lane stores its runs of RUN columns; at an edge sixteen rows at a time go through LDS
 // of the wave's own (16 rows of its columns) and are finished one by one, a row's columns side by side in the lanes.
-template <typename T, int EPI, uint32_t RUN, uint32_t S, uint32_t U>
+template <typename T, int EPI, int OUT, uint32_t RUN, uint32_t S, uint32_t U>
 __device__ __forceinline__ void finish_all(const Product& q, uint32_t m0, uint32_t n0, uint32_t split, const f32x4 (&acc)[S][U], float* lds) {
 	constexpr uint32_t WIDTH = U * 16u;
 	const uint32_t lane = threadIdx.x & 63u;
@@ -192,7 +206,7 @@ __device__ __forceinline__ void finish_all(const Product& q, uint32_t m0, uint32
 				float v[RUN];
 #pragma unroll
 				for (uint32_t r = 0; r < RUN; ++r) v[r] = acc[s][u + r / 4u][r % 4u];
-				finish<T, EPI>(q, m0 + s * 16u + lane % 16u, n0 + b_base<RUN>(u) + lane / 16u * RUN, split, v);
+				finish<T, EPI, OUT>(q, m0 + s * 16u + lane % 16u, n0 + b_base<RUN>(u) + lane / 16u * RUN, split, v);
 			}
 		return;
 	}
@@ -207,7 +221,7 @@ __device__ __forceinline__ void finish_all(const Product& q, uint32_t m0, uint32
 		for (uint32_t i = lane; i < 16u * WIDTH; i += 64u) {
 			const uint32_t m = m0 + s * 16u + i / WIDTH, n = n0 + i % WIDTH;
 			float v[1] = {mine[i]};
-			if (m < q.m && n < q.n) finish<T, EPI>(q, m, n, split, v);
+			if (m < q.m && n < q.n) finish<T, EPI, OUT>(q, m, n, split, v);
 		}
 		__builtin_amdgcn_wave_barrier();
 	}
@@ -215,7 +229,7 @@ __device__ __forceinline__ void finish_all(const Product& q, uint32_t m0, uint32
 
 // BM x BN of C to a workgroup, WM x WN waves.  The matrix instruction's rows are n and its columns m, so that a lane's four values stand side
 // by side in a row of C; where B is contiguous in k its rows are dealt to the instructions so that all of a lane's values do.
-template <typename T, bool A_KC, bool B_KC, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, int EPI>
+template <typename T, bool A_KC, bool B_KC, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, int EPI, int OUT>
 __device__ __forceinline__ void product(const Product& q, uint32_t block, uint4* __restrict__ tile_a, uint4* __restrict__ tile_b) {
 	constexpr uint32_t THREADS = WM * WN * 64u, S = BM / WM / 16u, U = BN / WN / 16u, RUN = B_KC ? 8u : 4u;
 	const uint32_t tile = block % (q.tiles_m * q.tiles_n), split = block / (q.tiles_m * q.tiles_n);
@@ -243,7 +257,7 @@ __device__ __forceinline__ void product(const Product& q, uint32_t block, uint4*
 		}
 		__syncthreads();
 	}
-	finish_all<T, EPI, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a));
+	finish_all<T, EPI, OUT, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a));
 }
 
 // The tile of load_tile straight from memory into LDS (no register in between): 16 bytes from each lane's address go to the wave's place and
@@ -314,7 +328,7 @@ __device__ __forceinline__ void product_stage(const uint4* __restrict__ ta, cons
 }
 
 // Two stages in LDS, 128 KiB, and eight waves of 128 x 64: a CU's LDS reads 96 of its 128 bytes a clock under full matrix cores.
-template <typename T, bool A_KC, bool B_KC, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, int EPI>
+template <typename T, bool A_KC, bool B_KC, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN, int EPI, int OUT>
 __device__ __forceinline__ void product_async(const Product& q, uint32_t block, uint32_t blocks, uint4* tile_a0, uint4* tile_a1, uint4* tile_b0, uint4* tile_b1) {
 	constexpr uint32_t THREADS = WM * WN * 64u, S = BM / WM / 16u, U = BN / WN / 16u, RUN = B_KC ? 8u : 4u;
 	const uint32_t tiles = q.tiles_m * q.tiles_n, work = n2_xcd_order(block, blocks), split = work / tiles;
@@ -351,14 +365,14 @@ __device__ __forceinline__ void product_async(const Product& q, uint32_t block, 
 		product_stage<T, A_KC, B_KC, BM, BN, RUN, THREADS>(tile_a0, tile_b0, tile_a1, tile_b1, 0u, a_read, b_read, a_tile, b_tile, acc);
 	}
 	__syncthreads();
-	finish_all<T, EPI, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a0));
+	finish_all<T, EPI, OUT, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a0));
 }
 
-template <typename T, bool ASYNC, bool A_KC, bool B_KC, uint32_t B, uint32_t WM, uint32_t WN, int EPI>
+template <typename T, bool ASYNC, bool A_KC, bool B_KC, uint32_t B, uint32_t WM, uint32_t WN, int EPI, int OUT>
 __global__ void __launch_bounds__(WM* WN * 64) product_kernel(Product q) {
 	__shared__ uint4 a0[B * BK / 8u], b0[B * BK / 8u], a1[ASYNC ? B * BK / 8u : 1u], b1[ASYNC ? B * BK / 8u : 1u];
-	if constexpr (ASYNC) product_async<T, A_KC, B_KC, B, B, WM, WN, EPI>(q, blockIdx.x, gridDim.x, a0, a1, b0, b1);
-	else product<T, A_KC, B_KC, B, B, WM, WN, EPI>(q, blockIdx.x, a0, b0);
+	if constexpr (ASYNC) product_async<T, A_KC, B_KC, B, B, WM, WN, EPI, OUT>(q, blockIdx.x, gridDim.x, a0, a1, b0, b1);
+	else product<T, A_KC, B_KC, B, B, WM, WN, EPI, OUT>(q, blockIdx.x, a0, b0);
 }
 
 // Both products of a backward pass in one launch, where they are small: the first blocks_x workgroups are dx's.
@@ -366,19 +380,18 @@ template <typename T, bool ASYNC>
 __global__ void __launch_bounds__(256) product_pair_kernel(Product x, Product w, uint32_t blocks_x) {
 	__shared__ uint4 a0[64u * BK / 8u], b0[64u * BK / 8u], a1[ASYNC ? 64u * BK / 8u : 1u], b1[ASYNC ? 64u * BK / 8u : 1u];
 	if (blockIdx.x < blocks_x) {
-		if constexpr (ASYNC) product_async<T, true, false, 64, 64, 2, 2, STORE>(x, blockIdx.x, blocks_x, a0, a1, b0, b1);
-		else product<T, true, false, 64, 64, 2, 2, STORE>(x, blockIdx.x, a0, b0);
+		if constexpr (ASYNC) product_async<T, true, false, 64, 64, 2, 2, STORE, EITHER>(x, blockIdx.x, blocks_x, a0, a1, b0, b1);
+		else product<T, true, false, 64, 64, 2, 2, STORE, EITHER>(x, blockIdx.x, a0, b0);
 	} else {
-		if constexpr (ASYNC) product_async<T, false, false, 64, 64, 2, 2, GRADIENT>(w, blockIdx.x - blocks_x, gridDim.x - blocks_x, a0, a1, b0, b1);
-		else product<T, false, false, 64, 64, 2, 2, GRADIENT>(w, blockIdx.x - blocks_x, a0, b0);
+		if constexpr (ASYNC) product_async<T, false, false, 64, 64, 2, 2, GRADIENT, EITHER>(w, blockIdx.x - blocks_x, gridDim.x - blocks_x, a0, a1, b0, b1);
+		else product<T, false, false, 64, 64, 2, 2, GRADIENT, EITHER>(w, blockIdx.x - blocks_x, a0, b0);
 	}
 }
 
 // The sums of the parts that k was dealt out to, finished: a lane takes four columns of a row.
 template <typename T, int EPI>
-__device__ __forceinline__ void join(Product q, uint32_t block) {
+__device__ __forceinline__ void join(const Product& q, uint32_t block) {
 	const float* partial = q.partial;
-	q.partial = nullptr;
 	const uint32_t quads = n2_ceil_div(q.n, 4u);
 	const uint64_t at = (uint64_t)block * 256u + threadIdx.x, row = at / quads;
 	if (row >= q.m) return;
@@ -393,12 +406,12 @@ __device__ __forceinline__ void join(Product q, uint32_t block) {
 			__builtin_memcpy(t, p + i * pitch, 16);
 			v[0] += t[0], v[1] += t[1], v[2] += t[2], v[3] += t[3];
 		}
-		finish<T, EPI>(q, m, n, 0u, v);
+		finish<T, EPI, WHOLE>(q, m, n, 0u, v);
 	} else {
 		for (uint32_t j = 0; j < valid; ++j) {
 			float w[1] = {0.f};
 			for (uint32_t i = 0; i < q.splits; ++i) w[0] += p[i * pitch + j];
-			finish<T, EPI>(q, m, n + j, 0u, w);
+			finish<T, EPI, WHOLE>(q, m, n + j, 0u, w);
 		}
 	}
 }
@@ -484,14 +497,19 @@ template <typename T, bool A_KC, bool B_KC, int EPI>
 int launch_product(hipStream_t s, const Product& q, uint32_t tile) {
 	N2_REQUIRE(blocks_of(q) <= 0xFFFFFFFFull / 512u, "n2_linear: %u x %u values take %llu workgroups", q.m, q.n, (unsigned long long)blocks_of(q));
 	const dim3 grid((uint32_t)blocks_of(q));
-	auto launch = [&](auto async) {
+	auto launch = [&](auto async, auto out) {
 		constexpr bool ASYNC = decltype(async)::value;
-		if (tile == 256) product_kernel<T, ASYNC, A_KC, B_KC, 256, 2, 4, EPI><<<grid, dim3(512), 0, s>>>(q);
-		else if (tile == 128) product_kernel<T, ASYNC, A_KC, B_KC, 128, 2, 2, EPI><<<grid, dim3(256), 0, s>>>(q);
-		else product_kernel<T, ASYNC, A_KC, B_KC, 64, 2, 2, EPI><<<grid, dim3(256), 0, s>>>(q);
+		constexpr int OUT = decltype(out)::value;
+		if (tile == 256) product_kernel<T, ASYNC, A_KC, B_KC, 256, 2, 4, EPI, OUT><<<grid, dim3(512), 0, s>>>(q);
+		else if (tile == 128) product_kernel<T, ASYNC, A_KC, B_KC, 128, 2, 2, EPI, OUT><<<grid, dim3(256), 0, s>>>(q);
+		else product_kernel<T, ASYNC, A_KC, B_KC, 64, 2, 2, EPI, OUT><<<grid, dim3(256), 0, s>>>(q);
 	};
-	if (async_product<A_KC, B_KC>(q)) launch(std::true_type{});
-	else launch(std::false_type{});
+	auto with_out = [&](auto async) {
+		if (q.partial != nullptr) launch(async, std::integral_constant<int, SPLIT>{});
+		else launch(async, std::integral_constant<int, WHOLE>{});
+	};
+	if (async_product<A_KC, B_KC>(q)) with_out(std::true_type{});
+	else with_out(std::false_type{});
 	N2_LAUNCH_CHECK();
 	return N2_OK;
 }
