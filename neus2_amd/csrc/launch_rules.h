@@ -325,6 +325,11 @@ static inline N2LinearPlan n2_linear_plan(uint32_t m, uint32_t n, uint32_t k) {
 }
 static inline uint64_t n2_linear_partial_bytes(const N2LinearPlan& plan, uint32_t m, uint32_t n) { return plan.splits > 1 ? 4ull * plan.splits * m * n : 0ull; }
 
+// Whether a forward pass has so few rows that its weights go straight into registers (few_rows_kernel).  GPU time in us, that way | in tiles:
+// 1 x 2048 x 2048 4.5 | 7.2, 8 x 4000 x 300 6.5 | 8.2, 16 x 2048 x 2048 5.9 | 8.7, 16 x 4096 x 4096 10.1 | 11.5, 16 x 333 x 77 4.9 | 10.4; two and four
+// instructions of rows 32 x 1024 x 1024 5.9 | 5.8, 32 x 4096 x 4096 13.9 | 11.4, 64 x 2048 x 2048 11.4 | 9.2, 64 x 4000 x 64 14.8 | 7.9.
+static inline bool n2_linear_few_rows(uint32_t m) { return m <= 16u; }
+
 // Workgroups that come one after the other go to the XCDs in turn: the number that makes consecutive work one XCD's, which then reads it
 // from its own L2.
 N2_HD inline uint32_t n2_xcd_order(uint32_t block, uint32_t blocks) {

@@ -430,6 +430,37 @@ __global__ void __launch_bounds__(256) join_backward_kernel(Product x, uint32_t 
 	else n2_column_sums_block<16, 1, 16>(sums, sum_rows, columns, block - blocks_x - blocks_w, [&](uint32_t column, float sum) { n2_store_sum(db + column, sum, accumulate); });
 }
 
+// A layer of up to sixteen rows: what it takes is the weights' way from memory, so sixteen columns of C go to a workgroup and its sixteen
+// waves take 32 values of k in turn, straight into the matrix instructions' registers; every wave's loads are under way at once.
+template <typename T>
+__global__ void __launch_bounds__(1024) few_rows_kernel(Product q) {
+	constexpr uint32_t WAVES = 16u, AT_ONCE = 4u;
+	__shared__ float part[WAVES][16u][16u];
+	const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u, i = lane % 16u, g = lane / 16u, n0 = blockIdx.x * 16u;
+	const T* w = static_cast<const T*>(q.b.p) + (uint64_t)min(n0 + i, q.n - 1u) * q.b.ld;
+	const T* x = static_cast<const T*>(q.a.p) + (uint64_t)min(i, q.m - 1u) * q.a.ld;
+	f32x4 acc = {};
+	for (uint32_t k0 = wave * 32u; k0 < q.k; k0 += WAVES * 32u * AT_ONCE) {
+		s16x8 b[AT_ONCE], a[AT_ONCE];
+#pragma unroll
+		for (uint32_t j = 0; j < AT_ONCE; ++j) {
+			const uint32_t k = k0 + j * WAVES * 32u + g * 8u, valid = k < q.k ? min(q.k - k, 8u) : 0u;
+			b[j] = __builtin_bit_cast(s16x8, n2_load_vec(w + k, valid));
+			a[j] = __builtin_bit_cast(s16x8, n2_load_vec(x + k, valid));
+		}
+#pragma unroll
+		for (uint32_t j = 0; j < AT_ONCE; ++j) acc = mfma(T{}, b[j], a[j], acc);
+	}
+	*reinterpret_cast<f32x4*>(&part[wave][i][g * 4u]) = acc;
+	__syncthreads();
+	const uint32_t m = threadIdx.x / 16u, n = threadIdx.x % 16u;
+	if (m >= q.m || m >= 16u || n0 + n >= q.n) return;
+	float v[1] = {0.f};
+#pragma unroll
+	for (uint32_t k = 0; k < WAVES; ++k) v[0] += part[k][m][n];
+	finish<T, LAYER, WHOLE>(q, m, n0 + n, 0u, v);
+}
+
 // -------------------------------------------------------------------------------------------------------------------------------------
 // dz = dy * act'(z), and its column sums
 // -------------------------------------------------------------------------------------------------------------------------------------
@@ -551,7 +582,7 @@ BackwardPlan backward_plan(uint32_t n_rows, uint32_t in_width, uint32_t out_widt
 	N2_REQUIRE((pointer) == nullptr || n_rows <= 1 || ((stride) >= (width) && n2_rows_fit(n_rows, stride)), name ": the stride of " what " is below the width %u or beyond memory", width)
 
 N2_API uint64_t n2_linear_forward_workspace_bytes(uint32_t n_rows, uint32_t in_width, uint32_t out_width) {
-	return n_rows == 0 || in_width == 0 || out_width == 0 ? 0u : n2_linear_partial_bytes(n2_linear_plan(n_rows, out_width, in_width), n_rows, out_width);
+	return n2_linear_few_rows(n_rows) || in_width == 0 || out_width == 0 ? 0u : n2_linear_partial_bytes(n2_linear_plan(n_rows, out_width, in_width), n_rows, out_width);
 }
 
 N2_API int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation activation, uint32_t n_rows, uint32_t in_width, uint32_t out_width, const void* d_weights,
@@ -577,10 +608,15 @@ N2_API int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation a
 	q.m = n_rows, q.n = out_width, q.k = in_width;
 	q.c = d_output, q.ldc = output_stride;
 	q.bias = d_bias, q.residual = d_residual, q.ldr = residual_stride, q.pre = d_pre_activation, q.ldp = pre_stride, q.activation = activation;
-	const N2LinearPlan plan = n2_linear_plan(n_rows, out_width, in_width);
+	const N2LinearPlan plan = n2_linear_few_rows(n_rows) ? N2LinearPlan{64, 1, in_width} : n2_linear_plan(n_rows, out_width, in_width);
 	plan_product(q, plan, static_cast<float*>(d_workspace));
 	return with_type(dtype, [&](auto t) -> int {
 		using T = decltype(t);
+		if (n2_linear_few_rows(n_rows)) {
+			few_rows_kernel<T><<<dim3(n2_ceil_div(out_width, 16u)), dim3(1024), 0, n2_stream(stream)>>>(q);
+			N2_LAUNCH_CHECK();
+			return N2_OK;
+		}
 		if (const int rc = launch_product<T, true, true, LAYER>(n2_stream(stream), q, plan.tile)) return rc;
 		if (q.partial != nullptr) {
 			join_kernel<T><<<dim3(join_blocks(q)), dim3(256), 0, n2_stream(stream)>>>(q);
