@@ -330,6 +330,17 @@ static inline uint64_t n2_linear_partial_bytes(const N2LinearPlan& plan, uint32_
 // instructions of rows 32 x 1024 x 1024 5.9 | 5.8, 32 x 4096 x 4096 13.9 | 11.4, 64 x 2048 x 2048 11.4 | 9.2, 64 x 4000 x 64 14.8 | 7.9.
 static inline bool n2_linear_few_rows(uint32_t m) { return m <= 16u; }
 
+// Whether a layer passes over its rows with the weights in LDS (stream_rows_kernel), and the workgroups of that launch, each with sixteen
+// waves of sixteen rows: one to a CU where the weights fill LDS or the registers of those waves do.  GPU time in us, that way | in tiles, plain
+// and with a residual: 262 144 x 256 x 256 63 | 77 and 99 | 133, 100 000 x 256 x 256 31 | 38 and 38 | 52, 32 768 x 256 x 256 17 | 13 and 21 | 15,
+// 262 144 x 64 x 64 13 | 16 and 18 | 20, 32 768 x 64 x 64 4.4 | 4.2 and 5.4 | 4.4, 262 144 x 64 x 256 30 | 45 and 70 | 101, 262 144 x 128 x 128 27 | 33 and
+// 40 | 43, 50 000 x 200 x 136 14 | 19 and 17 | 24, 16 384 x 200 x 136 11 | 9 and 12 | 11.
+static inline bool n2_linear_streams(uint32_t m, uint32_t n, uint32_t k) { return m >= 49152u && n <= 256u && k <= 256u; }
+static inline uint32_t n2_linear_stream_blocks(uint32_t m, uint32_t lds_bytes) {
+	const uint32_t needed = n2_ceil_div(m, 256u), most = lds_bytes > 65536u ? 256u : 512u;
+	return needed < most ? needed : most;
+}
+
 // Workgroups that come one after the other go to the XCDs in turn: the number that makes consecutive work one XCD's, which then reads it
 // from its own L2.
 N2_HD inline uint32_t n2_xcd_order(uint32_t block, uint32_t blocks) {

@@ -192,6 +192,29 @@ __device__ __forceinline__ void finish(const Product& q, uint32_t m, uint32_t n,
 	}
 }
 
+// The layer's epilogue for eight columns whose bias and residual are in registers.
+template <typename T, bool RESIDUAL>
+__device__ __forceinline__ void finish_with(const Product& q, uint32_t m, uint32_t n, float (&v)[8], const uint4& bias, const uint4& residual) {
+	auto add = [&](const uint4& u) __attribute__((always_inline)) {
+		const N2Vec<T> t = __builtin_bit_cast(N2Vec<T>, u);
+#pragma unroll
+		for (uint32_t i = 0; i < 8u; ++i) v[i] += (float)t.v[i];
+	};
+	auto store = [&](void* p, uint64_t ld) __attribute__((always_inline)) {
+		N2Vec<T> t;
+#pragma unroll
+		for (uint32_t i = 0; i < 8u; ++i) t.v[i] = (T)v[i];
+		__builtin_memcpy(static_cast<T*>(p) + (uint64_t)m * ld + n, &t, 16);
+	};
+	if (q.bias != nullptr) add(bias);
+	if (q.pre != nullptr) store(q.pre, q.ldp);
+	if (q.activation != N2_ACTIVATION_NONE)
+#pragma unroll
+		for (uint32_t i = 0; i < 8u; ++i) v[i] = activation(v[i], q.activation);
+	if constexpr (RESIDUAL) add(residual);
+	store(q.c, q.ldc);
+}
+
 // What a wave has of C, from (m0, n0) on.  Inside C a lane stores its runs of RUN columns; at an edge sixteen rows at a time go through LDS
 // of the wave's own (16 rows of its columns) and are finished one by one, a row's columns side by side in the lanes.
 template <typename T, int EPI, int OUT, uint32_t RUN, uint32_t S, uint32_t U>
@@ -461,6 +484,84 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(Product q) {
 	finish<T, LAYER, WHOLE>(q, m, n0 + n, 0u, v);
 }
 
+// A layer of many rows and few columns: memory bounds it, and tiles that load, multiply and store in turn leave memory idle.  Here the
+// weights stay in LDS as the matrix instructions take them, and every wave passes over rows on its own, sixteen at a time: the next rows
+// come into registers while these are multiplied, and nothing is waited for in common.  KT steps of 32 values of k, NT instructions of 16
+// columns; widths and strides are multiples of eight, rows start at multiples of 16 bytes.  2^18 x 256 x 256: 4.2 TB/s, with a residual 4.1.
+// (32 rows to a wave halve what is read from LDS, and were no faster: 64 and 105 us for 63 and 99.)
+template <typename T, uint32_t KT, uint32_t NT, bool RESIDUAL>
+__global__ void __launch_bounds__(1024) stream_rows_kernel(Product q) {
+	__shared__ uint4 weights[NT * KT * 64u], bias[NT * 2u];
+	const uint32_t lane = threadIdx.x & 63u, i = lane % 16u, g = lane / 16u;
+	// (all of a lane's loads are under way at once)
+	constexpr uint32_t FILL = (NT * KT * 64u + 1023u) / 1024u;
+	uint4 fill[FILL];
+#pragma unroll
+	for (uint32_t j = 0; j < FILL; ++j) {
+		const uint32_t at = j * 1024u + threadIdx.x, u = at / 64u / KT, kk = at / 64u % KT, n = b_base<8>(u) + i / 4u * 8u + i % 4u, k = kk * 32u + g * 8u;
+		fill[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(q.b.p) + (uint64_t)min(n, q.n - 1u) * q.b.ld + min(k, q.k - 8u));
+		if (n >= q.n || k >= q.k) fill[j] = make_uint4(0u, 0u, 0u, 0u);
+	}
+#pragma unroll
+	for (uint32_t j = 0; j < FILL; ++j)
+		if (j * 1024u + threadIdx.x < NT * KT * 64u) weights[j * 1024u + threadIdx.x] = fill[j];
+	if (threadIdx.x < NT * 2u && threadIdx.x * 8u < q.n && q.bias != nullptr) bias[threadIdx.x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(q.bias) + threadIdx.x * 8u);
+	__syncthreads();
+	const uint64_t tiles = n2_ceil_div(q.m, 16u), step = (uint64_t)gridDim.x * 16u;
+	const T* x = static_cast<const T*>(q.a.p);
+	const T* r = static_cast<const T*>(q.residual);
+	auto load_x = [&](uint4 (&to)[KT], uint64_t tile) __attribute__((always_inline)) {
+		const uint64_t row = min(tile * 16u + i, (uint64_t)q.m - 1u);
+#pragma unroll
+		for (uint32_t kk = 0; kk < KT; ++kk) {
+			const uint32_t k = kk * 32u + g * 8u;
+			to[kk] = k < q.k ? *reinterpret_cast<const uint4*>(x + row * q.a.ld + k) : make_uint4(0u, 0u, 0u, 0u);
+		}
+	};
+	// (with a residual the registers hold its rows instead of the next ones of x)
+	constexpr uint32_t AHEAD = NT / 2u < 4u ? NT / 2u : 4u;
+	uint4 now[KT], next[RESIDUAL ? 1u : KT], add[RESIDUAL ? AHEAD : 1u];
+	uint64_t tile = (uint64_t)blockIdx.x * 16u + threadIdx.x / 64u;
+	if constexpr (!RESIDUAL)
+		if (tile < tiles) load_x(next, tile);
+	for (; tile < tiles; tile += step) {
+		const uint64_t m = tile * 16u + i;
+		auto load_r = [&](uint32_t u) __attribute__((always_inline)) {
+			const uint32_t n = b_base<8>(u) + g * 8u;
+			if (n < q.n) add[u / 2u % AHEAD] = *reinterpret_cast<const uint4*>(r + min(m, (uint64_t)q.m - 1u) * q.ldr + n);
+		};
+		if constexpr (RESIDUAL) {
+			load_x(now, tile);
+#pragma unroll
+			for (uint32_t u = 0; u < 2u * AHEAD; u += 2u) load_r(u);
+		} else {
+#pragma unroll
+			for (uint32_t kk = 0; kk < KT; ++kk) now[kk] = next[kk];
+			if (tile + step < tiles) load_x(next, tile + step);
+		}
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (uint32_t u = 0; u < NT; u += 2u) {
+			f32x4 acc[2] = {};
+#pragma unroll
+			for (uint32_t kk = 0; kk < KT; ++kk)
+#pragma unroll
+				for (uint32_t h = 0; h < 2u; ++h)
+					acc[h] = mfma(T{}, __builtin_bit_cast(s16x8, weights[((u + h) * KT + kk) * 64u + lane]), __builtin_bit_cast(s16x8, now[kk]), acc[h]);
+			const uint32_t n = b_base<8>(u) + g * 8u;
+			if (n < q.n && m < q.m) {
+				float v[8];
+#pragma unroll
+				for (uint32_t j = 0; j < 8u; ++j) v[j] = acc[j / 4u][j % 4u];
+				finish_with<T, RESIDUAL>(q, (uint32_t)m, n, v, bias[n / 8u], add[RESIDUAL ? u / 2u % AHEAD : 0u]);
+			}
+			if constexpr (RESIDUAL)
+				if (u + 2u * AHEAD < NT) load_r(u + 2u * AHEAD);
+			__builtin_amdgcn_sched_barrier(0);
+		}
+	}
+}
+
 // -------------------------------------------------------------------------------------------------------------------------------------
 // dz = dy * act'(z), and its column sums
 // -------------------------------------------------------------------------------------------------------------------------------------
@@ -545,6 +646,23 @@ int launch_product(hipStream_t s, const Product& q, uint32_t tile) {
 	return N2_OK;
 }
 
+// rows of whole vectors of eight values at multiples of 16 bytes (or nothing at all)
+bool rows_of_vectors(const void* p, uint64_t stride, uint32_t width) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0 && width % 8 == 0); }
+
+// f(steps of 32 values of k, instructions of 16 columns) for widths up to 256
+template <typename F>
+void with_narrow(uint32_t k, uint32_t n, F&& f) {
+	using std::integral_constant;
+	auto with_n = [&](auto kt) {
+		if (n <= 64u) f(kt, integral_constant<uint32_t, 4>{});
+		else if (n <= 128u) f(kt, integral_constant<uint32_t, 8>{});
+		else f(kt, integral_constant<uint32_t, 16>{});
+	};
+	if (k <= 64u) with_n(integral_constant<uint32_t, 2>{});
+	else if (k <= 128u) with_n(integral_constant<uint32_t, 4>{});
+	else with_n(integral_constant<uint32_t, 8>{});
+}
+
 template <typename F>
 int with_type(n2_dtype dtype, F&& f) {
 	return dtype == N2_DTYPE_F16 ? f(n2_f16{}) : f(n2_bf16{});
@@ -612,6 +730,18 @@ N2_API int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation a
 	plan_product(q, plan, static_cast<float*>(d_workspace));
 	return with_type(dtype, [&](auto t) -> int {
 		using T = decltype(t);
+		if (n2_linear_streams(n_rows, out_width, in_width) && async_product<true, true>(q) && rows_of_vectors(d_bias, 8, out_width) && rows_of_vectors(d_residual, residual_stride, out_width) &&
+		    rows_of_vectors(d_output, output_stride, out_width) && rows_of_vectors(d_pre_activation, pre_stride, out_width)) {
+			auto launch = [&](auto kt, auto nt) {
+				constexpr uint32_t KT = decltype(kt)::value, NT = decltype(nt)::value;
+				const dim3 grid(n2_linear_stream_blocks(n_rows, KT * NT * 1024u));
+				if (d_residual != nullptr) stream_rows_kernel<T, KT, NT, true><<<grid, dim3(1024), 0, n2_stream(stream)>>>(q);
+				else stream_rows_kernel<T, KT, NT, false><<<grid, dim3(1024), 0, n2_stream(stream)>>>(q);
+			};
+			with_narrow(in_width, out_width, launch);
+			N2_LAUNCH_CHECK();
+			return N2_OK;
+		}
 		if (n2_linear_few_rows(n_rows)) {
 			few_rows_kernel<T><<<dim3(n2_ceil_div(out_width, 16u)), dim3(1024), 0, n2_stream(stream)>>>(q);
 			N2_LAUNCH_CHECK();

@@ -40,7 +40,7 @@ def _linear(gen, i, o, kind, bias, dtype):
 
 # rows, in, out, extra columns, first column
 SHAPES = [(1, 1, 1, 0, 0), (1, 256, 256, 0, 0), (2, 3, 5, 3, 1), (16, 512, 96, 8, 8), (17, 200, 33, 0, 0), (64, 64, 64, 0, 0), (65, 63, 129, 1, 1), (128, 128, 128, 0, 0),
-          (130, 257, 31, 0, 0), (300, 72, 257, 8, 0), (513, 320, 257, 7, 3), (1000, 40, 24, 0, 0), (257, 1032, 264, 0, 0), (1500, 16, 8, 0, 0), (700, 500, 300, 4, 4)]
+          (130, 257, 31, 0, 0), (300, 72, 257, 8, 0), (513, 320, 257, 7, 3), (1000, 40, 24, 0, 0), (257, 1032, 264, 0, 0), (1500, 16, 8, 0, 0), (700, 500, 300, 4, 4), (20, 2056, 64, 0, 0), (33, 1000, 136, 8, 8)]
 
 
 @pytest.mark.parametrize("dtype", HALVES)
@@ -108,6 +108,25 @@ def test_linear_backward_sums_many_rows(n, i, o, dtype):
     ref.within(grads[o * i:], *e["db"], "db")
     op._grads.zero_()
     assert torch.equal(op.backward(x, z, dy), dx) and torch.equal(op._grads, grads)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("n,i,o,residual,kind", [(49152, 256, 256, True, "None"), (49155, 64, 64, False, "SiLU"), (50001, 200, 136, True, "GELU"), (60000, 8, 8, False, "None"), (50000, 72, 256, True, "ReLU"),
+                                                 (70001, 128, 24, False, "GELU"), (49200, 256, 64, True, "SiLU"), (49200, 40, 128, True, "None"), (49153, 36, 68, True, "None")])
+def test_linear_forward_of_many_rows(n, i, o, residual, kind, dtype):
+    """Narrow layers of many rows keep their weights in LDS and pass over the rows: widths inside their steps, ragged last rows, the residual in place."""
+    gen = torch.Generator().manual_seed(n + i)
+    op, w, b = _linear(gen, i, o, kind, bias=i != 64, dtype=dtype)
+    x, r = _rows(gen, n, i, dtype, 8, 8), _rows(gen, n, o, dtype) if residual else None
+    out, check = _canvas(n, o, dtype, 16, 8)
+    y, z = op.forward(x, residual=r, want_pre_activation=True, out=out)
+    ye, ze, dy, dz = ref.linear_forward(x, w, b, r, kind)
+    ref.within(y, ye, dy, "y")
+    ref.within(z, ze, dz, "z")
+    check()
+    if residual:
+        op.forward(x, residual=r, out=r)
+        assert torch.equal(r, y)
 
 
 @pytest.mark.parametrize("dtype", HALVES)
@@ -332,7 +351,7 @@ def _gradients(gen, sizes, dtypes, scale=1.0):
 ALL = [torch.float16, torch.bfloat16, torch.float32]
 
 
-@pytest.mark.parametrize("sizes", [[1], [7, 0, 8193], [8192] * 3, [100003, 3, 64, 16385, 1], [5] * 700])
+@pytest.mark.parametrize("sizes", [[1], [7, 0, 8193], [8192] * 3, [100003, 3, 64, 16385, 1], [5] * 700, [9000001, 2049, 17, 4097]])
 @pytest.mark.parametrize("dtypes", [[t] for t in ALL] + [ALL])
 @pytest.mark.parametrize("apart", [False, True])
 def test_clip(sizes, dtypes, apart):
