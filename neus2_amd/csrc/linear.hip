@@ -489,22 +489,42 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(Product q) {
 // come into registers while these are multiplied, and nothing is waited for in common.  KT steps of 32 values of k, NT instructions of 16
 // columns; widths and strides are multiples of eight, rows start at multiples of 16 bytes.  2^18 x 256 x 256: 4.2 TB/s, with a residual 4.1.
 // (32 rows to a wave halve what is read from LDS, and were no faster: 64 and 105 us for 63 and 99.)
-template <typename T, uint32_t KT, uint32_t NT, bool RESIDUAL>
+template <typename T, uint32_t KT, uint32_t NT, bool RESIDUAL, bool B_KC>
 __global__ void __launch_bounds__(1024) stream_rows_kernel(Product q) {
 	__shared__ uint4 weights[NT * KT * 64u], bias[NT * 2u];
 	const uint32_t lane = threadIdx.x & 63u, i = lane % 16u, g = lane / 16u;
 	// (all of a lane's loads are under way at once)
-	constexpr uint32_t FILL = (NT * KT * 64u + 1023u) / 1024u;
-	uint4 fill[FILL];
+	if constexpr (B_KC) {
+		constexpr uint32_t FILL = (NT * KT * 64u + 1023u) / 1024u;
+		uint4 fill[FILL];
+	#pragma unroll
+		for (uint32_t j = 0; j < FILL; ++j) {
+			const uint32_t at = j * 1024u + threadIdx.x, u = at / 64u / KT, kk = at / 64u % KT, n = b_base<8>(u) + i / 4u * 8u + i % 4u, k = kk * 32u + g * 8u;
+			fill[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(q.b.p) + (uint64_t)min(n, q.n - 1u) * q.b.ld + min(k, q.k - 8u));
+			if (n >= q.n || k >= q.k) fill[j] = make_uint4(0u, 0u, 0u, 0u);
+		}
+	#pragma unroll
+		for (uint32_t j = 0; j < FILL; ++j)
+			if (j * 1024u + threadIdx.x < NT * KT * 64u) weights[j * 1024u + threadIdx.x] = fill[j];
+	} else {
+		// columns of W as rows: eight by eight values to a lane, turned around in its registers
+		static_assert(NT * KT * 8u <= 1024u, "");
+		const uint32_t n = threadIdx.x % (NT * 2u) * 8u, k = threadIdx.x / (NT * 2u) * 8u;
+		N2Vec<T> in[8];
 #pragma unroll
-	for (uint32_t j = 0; j < FILL; ++j) {
-		const uint32_t at = j * 1024u + threadIdx.x, u = at / 64u / KT, kk = at / 64u % KT, n = b_base<8>(u) + i / 4u * 8u + i % 4u, k = kk * 32u + g * 8u;
-		fill[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(q.b.p) + (uint64_t)min(n, q.n - 1u) * q.b.ld + min(k, q.k - 8u));
-		if (n >= q.n || k >= q.k) fill[j] = make_uint4(0u, 0u, 0u, 0u);
+		for (uint32_t j = 0; j < 8u; ++j) {
+			const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(q.b.p) + (uint64_t)min(k + j, q.k - 1u) * q.b.ld + min(n, q.n - 8u));
+			in[j] = __builtin_bit_cast(N2Vec<T>, n < q.n && k + j < q.k ? u : make_uint4(0u, 0u, 0u, 0u));
+		}
+		if (k < KT * 32u)
+#pragma unroll
+			for (uint32_t e = 0; e < 8u; ++e) {
+				N2Vec<T> out;
+#pragma unroll
+				for (uint32_t j = 0; j < 8u; ++j) out.v[j] = in[j].v[e];
+				weights[((n / 32u * 2u + e / 4u) * KT + k / 32u) * 64u + k % 32u / 8u * 16u + n % 32u / 8u * 4u + e % 4u] = __builtin_bit_cast(uint4, out);
+			}
 	}
-#pragma unroll
-	for (uint32_t j = 0; j < FILL; ++j)
-		if (j * 1024u + threadIdx.x < NT * KT * 64u) weights[j * 1024u + threadIdx.x] = fill[j];
 	if (threadIdx.x < NT * 2u && threadIdx.x * 8u < q.n && q.bias != nullptr) bias[threadIdx.x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(q.bias) + threadIdx.x * 8u);
 	__syncthreads();
 	const uint64_t tiles = n2_ceil_div(q.m, 16u), step = (uint64_t)gridDim.x * 16u;
@@ -735,8 +755,8 @@ N2_API int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation a
 			auto launch = [&](auto kt, auto nt) {
 				constexpr uint32_t KT = decltype(kt)::value, NT = decltype(nt)::value;
 				const dim3 grid(n2_linear_stream_blocks(n_rows, KT * NT * 1024u));
-				if (d_residual != nullptr) stream_rows_kernel<T, KT, NT, true><<<grid, dim3(1024), 0, n2_stream(stream)>>>(q);
-				else stream_rows_kernel<T, KT, NT, false><<<grid, dim3(1024), 0, n2_stream(stream)>>>(q);
+				if (d_residual != nullptr) stream_rows_kernel<T, KT, NT, true, true><<<grid, dim3(1024), 0, n2_stream(stream)>>>(q);
+				else stream_rows_kernel<T, KT, NT, false, true><<<grid, dim3(1024), 0, n2_stream(stream)>>>(q);
 			};
 			with_narrow(in_width, out_width, launch);
 			N2_LAUNCH_CHECK();
@@ -832,8 +852,16 @@ N2_API int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation 
 			else product_pair_kernel<T, false><<<grid, dim3(256), 0, s>>>(x, w, (uint32_t)blocks_of(x));
 			N2_LAUNCH_CHECK();
 		} else {
-			if (has_x)
+			if (has_x && n2_linear_streams(n_rows, in_width, out_width) && async && x.k % 8 == 0 && rows_of_vectors(d_dL_dinput, dL_dinput_stride, in_width)) {
+				with_narrow(out_width, in_width, [&](auto kt, auto nt) {
+					constexpr uint32_t KT = decltype(kt)::value, NT = decltype(nt)::value;
+					stream_rows_kernel<T, KT, NT, false, false><<<dim3(n2_linear_stream_blocks(n_rows, KT * NT * 1024u)), dim3(1024), 0, s>>>(x);
+				});
+				N2_LAUNCH_CHECK();
+				x.partial = nullptr;
+			} else if (has_x) {
 				if (const int rc = launch_product<T, true, false, STORE>(s, x, p.input.tile)) return rc;
+			}
 			if (dw != nullptr)
 				if (const int rc = launch_product<T, false, false, GRADIENT>(s, w, p.weights.tile)) return rc;
 		}
