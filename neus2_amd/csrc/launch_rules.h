@@ -271,14 +271,14 @@ static inline N2GatherGrid n2_rows_of_blocks(uint32_t blocks, uint32_t threads) 
 }
 
 // Workgroups of a layer norm's launch, each taking groups of rows as far apart as there are workgroups.  Backward, where each leaves two rows
-// of fp32 sums: at least eight rows to one beyond the first 256.
+// of fp32 sums: at least four rows to one beyond the first 256.
 static inline uint32_t n2_layer_norm_forward_blocks(uint32_t n_rows, uint32_t rows_per_block, uint32_t threads) {
 	const uint32_t needed = n_rows / rows_per_block + (n_rows % rows_per_block != 0u), most = threads > 256u ? 512u : 2048u;
 	return needed < most ? needed : most;
 }
 static inline uint32_t n2_layer_norm_backward_blocks(uint32_t n_rows, uint32_t rows_per_block, uint32_t threads) {
 	const uint32_t needed = n_rows / rows_per_block + (n_rows % rows_per_block != 0u), top = threads > 256u ? 512u : 1024u;
-	const uint32_t some = n_rows / 8u > 256u ? n_rows / 8u : 256u, most = some < top ? some : top;
+	const uint32_t some = n_rows / 4u > 256u ? n_rows / 4u : 256u, most = some < top ? some : top;
 	return needed < most ? needed : most;
 }
 
@@ -315,10 +315,10 @@ static inline N2LinearPlan n2_linear_plan(uint32_t m, uint32_t n, uint32_t k) {
 	const double tiles = (double)tiles_of(64);
 	uint32_t best = 1;
 	double least = 0.;
-	constexpr uint32_t tried[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
+	constexpr uint32_t tried[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512};
 	for (uint32_t s : tried) {
 		if (s > 1u && (2u * s > stages || tiles * s > 1024.)) break;
-		const double turns = tiles * s / 512., us = 0.45 * stages / s * (turns > 1. ? turns : 1.) + (s > 1u ? 2. + 0.06 * s + s * ((double)m * n) * 8. / 3e6 : 0.);
+		const double turns = tiles * s / 512., us = 0.45 * stages / s * (turns > 1. ? turns : 1.) + (s > 1u ? 2. + 0.05 * s + s * ((double)m * n) * 8. / 3e6 : 0.);
 		if (s == 1u || us < least) best = s, least = us;
 	}
 	return split(64, best, best);

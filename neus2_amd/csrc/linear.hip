@@ -411,34 +411,50 @@ __global__ void __launch_bounds__(256) product_pair_kernel(Product x, Product w,
 	}
 }
 
-// The sums of the parts that k was dealt out to, finished: a lane takes four columns of a row.
+// The sums of the parts that k was dealt out to, finished: a lane takes four columns of a row, and of many parts every sixteenth.
+constexpr uint32_t JOIN_ALONE = 16;
 template <typename T, int EPI>
 __device__ __forceinline__ void join(const Product& q, uint32_t block) {
-	const float* partial = q.partial;
-	const uint32_t quads = n2_ceil_div(q.n, 4u);
-	const uint64_t at = (uint64_t)block * 256u + threadIdx.x, row = at / quads;
-	if (row >= q.m) return;
-	const uint32_t m = (uint32_t)row, n = (uint32_t)(at - row * quads) * 4u, valid = min(q.n - n, 4u);
-	float v[4] = {0.f, 0.f, 0.f, 0.f};
-	const float* p = partial + row * q.n + n;
+	__shared__ f32x4 part[16][16];
+	const bool alone = q.splits <= JOIN_ALONE;
+	const uint32_t quads = n2_ceil_div(q.n, 4u), first = alone ? 0u : threadIdx.x / 16u, step = alone ? 1u : 16u;
+	const uint64_t at = alone ? (uint64_t)block * 256u + threadIdx.x : (uint64_t)block * 16u + threadIdx.x % 16u, row = at / quads;
+	const uint32_t m = (uint32_t)row, n = (uint32_t)(at - row * quads) * 4u, valid = row < q.m ? min(q.n - n, 4u) : 0u;
+	f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+	const float* p = q.partial + row * q.n + n;
 	const uint64_t pitch = (uint64_t)q.m * q.n;
 	if (valid == 4u) {
 #pragma unroll 8
-		for (uint32_t i = 0; i < q.splits; ++i) {
-			float t[4];
-			__builtin_memcpy(t, p + i * pitch, 16);
-			v[0] += t[0], v[1] += t[1], v[2] += t[2], v[3] += t[3];
+		for (uint32_t i = first; i < q.splits; i += step) {
+			f32x4 t;
+			__builtin_memcpy(&t, p + i * pitch, 16);
+			sum += t;
 		}
+	} else {
+		for (uint32_t i = first; i < q.splits; i += step)
+#pragma unroll
+			for (uint32_t j = 0; j < 3u; ++j)
+				if (j < valid) sum[j] += p[i * pitch + j];
+	}
+	if (!alone) {
+		part[first][threadIdx.x % 16u] = sum;
+		__syncthreads();
+		if (first != 0u) return;
+#pragma unroll
+		for (uint32_t i = 1; i < 16u; ++i) sum += part[i][threadIdx.x];
+	}
+	if (valid == 4u) {
+		float v[4] = {sum[0], sum[1], sum[2], sum[3]};
 		finish<T, EPI, WHOLE>(q, m, n, 0u, v);
 	} else {
-		for (uint32_t j = 0; j < valid; ++j) {
-			float w[1] = {0.f};
-			for (uint32_t i = 0; i < q.splits; ++i) w[0] += p[i * pitch + j];
-			finish<T, EPI, WHOLE>(q, m, n + j, 0u, w);
+#pragma unroll
+		for (uint32_t j = 0; j < 3u; ++j) {
+			float v[1] = {sum[j]};
+			if (j < valid) finish<T, EPI, WHOLE>(q, m, n + j, 0u, v);
 		}
 	}
 }
-uint32_t join_blocks(const Product& q) { return q.partial != nullptr ? n2_ceil_div((uint64_t)q.m * n2_ceil_div(q.n, 4u), 256u) : 0u; }
+uint32_t join_blocks(const Product& q) { return q.partial != nullptr ? n2_ceil_div((uint64_t)q.m * n2_ceil_div(q.n, 4u), q.splits <= JOIN_ALONE ? 256u : 16u) : 0u; }
 
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(Product q) { join<T, LAYER>(q, blockIdx.x); }
