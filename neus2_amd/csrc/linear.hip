@@ -49,6 +49,29 @@ __device__ __forceinline__ float activation_slope(float z, int kind) {
 	return 1.f;
 }
 
+__device__ __forceinline__ float slope_times(float dy, float z, int kind) {
+	if (kind == N2_ACTIVATION_NONE) return dy;
+	if (kind == N2_ACTIVATION_RELU) return z > 0.f ? dy : 0.f;
+	return dy * activation_slope(z, kind);
+}
+
+// Eight values in each of sixteen lanes, i their number: the sum of value i % 8 over all lanes.  Each step keeps the half of the values that the
+// lane's next bit names and takes the partner's: 8, 4, 2 and 1 are left.
+__device__ __forceinline__ float sum_of_sixteen(float (&v)[8], uint32_t i) {
+	auto dpp = [](float x, auto control) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(control)::value, 0xf, 0xf, true)); };
+	auto half = [&](uint32_t n, uint32_t bit, auto control) __attribute__((always_inline)) {
+#pragma unroll
+		for (uint32_t j = 0; j < n; ++j) {
+			const float low = v[j], high = v[j + n];
+			v[j] = ((i & bit) != 0u ? high : low) + dpp((i & bit) != 0u ? low : high, control);
+		}
+	};
+	half(4u, 4u, std::integral_constant<int, 0x141>{});  // row_half_mirror: lane i ^ 7
+	half(2u, 2u, std::integral_constant<int, 0x1B>{});   // quad_perm 3 2 1 0: i ^ 3
+	half(1u, 1u, std::integral_constant<int, 0xB1>{});   // quad_perm 1 0 3 2: i ^ 1
+	return v[0] + dpp(v[0], std::integral_constant<int, 0x128>{});  // row_ror 8: i ^ 8
+}
+
 // -------------------------------------------------------------------------------------------------------------------------------------
 // tiles
 // -------------------------------------------------------------------------------------------------------------------------------------
@@ -500,14 +523,10 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(Product q) {
 	finish<T, LAYER, WHOLE>(q, m, n0 + n, 0u, v);
 }
 
-// A layer of many rows and few columns: memory bounds it, and tiles that load, multiply and store in turn leave memory idle.  Here the
-// weights stay in LDS as the matrix instructions take them, and every wave passes over rows on its own, sixteen at a time: the next rows
-// come into registers while these are multiplied, and nothing is waited for in common.  KT steps of 32 values of k, NT instructions of 16
-// columns; widths and strides are multiples of eight, rows start at multiples of 16 bytes.  2^18 x 256 x 256: 4.2 TB/s, with a residual 4.1.
-// (32 rows to a wave halve what is read from LDS, and were no faster: 64 and 105 us for 63 and 99.)
-template <typename T, uint32_t KT, uint32_t NT, bool RESIDUAL, bool B_KC>
-__global__ void __launch_bounds__(1024) stream_rows_kernel(Product q) {
-	__shared__ uint4 weights[NT * KT * 64u], bias[NT * 2u];
+// The weights of a narrow layer in LDS, as the matrix instructions take them: KT steps of 32 values of k, NT instructions of 16 columns, whose
+// pairs leave eight consecutive columns of C in a lane.
+template <typename T, uint32_t KT, uint32_t NT, bool B_KC>
+__device__ __forceinline__ void fill_weights(const Product& q, uint4* weights) {
 	const uint32_t lane = threadIdx.x & 63u, i = lane % 16u, g = lane / 16u;
 	// (all of a lane's loads are under way at once)
 	if constexpr (B_KC) {
@@ -541,6 +560,18 @@ __global__ void __launch_bounds__(1024) stream_rows_kernel(Product q) {
 				weights[((n / 32u * 2u + e / 4u) * KT + k / 32u) * 64u + k % 32u / 8u * 16u + n % 32u / 8u * 4u + e % 4u] = __builtin_bit_cast(uint4, out);
 			}
 	}
+}
+
+// A layer of many rows and few columns: memory bounds it, and tiles that load, multiply and store in turn leave memory idle.  Here the
+// weights stay in LDS as the matrix instructions take them, and every wave passes over rows on its own, sixteen at a time: the next rows
+// come into registers while these are multiplied, and nothing is waited for in common.  KT steps of 32 values of k, NT instructions of 16
+// columns; widths and strides are multiples of eight, rows start at multiples of 16 bytes.  2^18 x 256 x 256: 4.2 TB/s, with a residual 4.1.
+// (32 rows to a wave halve what is read from LDS, and were no faster: 64 and 105 us for 63 and 99.)
+template <typename T, uint32_t KT, uint32_t NT, bool RESIDUAL>
+__global__ void __launch_bounds__(1024) stream_rows_kernel(Product q) {
+	__shared__ uint4 weights[NT * KT * 64u], bias[NT * 2u];
+	const uint32_t lane = threadIdx.x & 63u, i = lane % 16u, g = lane / 16u;
+	fill_weights<T, KT, NT, true>(q, weights);
 	if (threadIdx.x < NT * 2u && threadIdx.x * 8u < q.n && q.bias != nullptr) bias[threadIdx.x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(q.bias) + threadIdx.x * 8u);
 	__syncthreads();
 	const uint64_t tiles = n2_ceil_div(q.m, 16u), step = (uint64_t)gridDim.x * 16u;
@@ -598,6 +629,79 @@ __global__ void __launch_bounds__(1024) stream_rows_kernel(Product q) {
 	}
 }
 
+// dx of a narrow layer of many rows in the same way.  q.a is dz, or dy, with z (or null, without an activation): then dz is formed in the
+// registers that the matrix instructions take it from.  partial (or null): its column sums, one row of q.k from each workgroup.
+template <typename T, uint32_t KT, uint32_t NT>
+__global__ void __launch_bounds__(1024) stream_backward_kernel(Product q, const T* __restrict__ z, uint64_t ld_z, float* __restrict__ partial) {
+	__shared__ uint4 weights[NT * KT * 64u];
+	const uint32_t lane = threadIdx.x & 63u, i = lane % 16u, g = lane / 16u, wave = threadIdx.x / 64u;
+	fill_weights<T, KT, NT, false>(q, weights);
+	__syncthreads();
+	const uint64_t tiles = n2_ceil_div(q.m, 16u), step = (uint64_t)gridDim.x * 16u;
+	const T* dy = static_cast<const T*>(q.a.p);
+	float sums[KT] = {};  // of column kk * 32 + g * 8 + i % 8, over the lanes of a row of sixteen
+	for (uint64_t tile = (uint64_t)blockIdx.x * 16u + wave; tile < tiles; tile += step) {
+		const uint64_t m = tile * 16u + i, row = min(m, (uint64_t)q.m - 1u);
+		uint4 now[KT], pre[KT];
+#pragma unroll
+		for (uint32_t kk = 0; kk < KT; ++kk) {
+			const uint32_t k = kk * 32u + g * 8u;
+			now[kk] = pre[kk] = make_uint4(0u, 0u, 0u, 0u);
+			if (k < q.k) {
+				now[kk] = *reinterpret_cast<const uint4*>(dy + row * q.a.ld + k);
+				if (z != nullptr) pre[kk] = *reinterpret_cast<const uint4*>(z + row * ld_z + k);
+			}
+		}
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (uint32_t kk = 0; kk < KT; ++kk) {
+			if (z == nullptr && partial == nullptr) break;
+			const N2Vec<T> d = __builtin_bit_cast(N2Vec<T>, now[kk]), p = __builtin_bit_cast(N2Vec<T>, pre[kk]);
+			float v[8];
+			N2Vec<T> out;
+#pragma unroll
+			for (uint32_t j = 0; j < 8u; ++j) {
+				v[j] = slope_times((float)d.v[j], (float)p.v[j], z != nullptr ? q.activation : N2_ACTIVATION_NONE);
+				out.v[j] = (T)v[j];
+				v[j] = m < q.m ? v[j] : 0.f;
+			}
+			now[kk] = __builtin_bit_cast(uint4, out);
+			if (partial != nullptr) sums[kk] += sum_of_sixteen(v, i);
+		}
+#pragma unroll
+		for (uint32_t u = 0; u < NT; u += 2u) {
+			f32x4 acc[2] = {};
+#pragma unroll
+			for (uint32_t kk = 0; kk < KT; ++kk)
+#pragma unroll
+				for (uint32_t h = 0; h < 2u; ++h)
+					acc[h] = mfma(T{}, __builtin_bit_cast(s16x8, weights[((u + h) * KT + kk) * 64u + lane]), __builtin_bit_cast(s16x8, now[kk]), acc[h]);
+			const uint32_t n = b_base<8>(u) + g * 8u;
+			if (n < q.n && m < q.m) {
+				N2Vec<T> out;
+#pragma unroll
+				for (uint32_t j = 0; j < 8u; ++j) out.v[j] = (T)acc[j / 4u][j % 4u];
+				__builtin_memcpy(static_cast<T*>(q.c) + m * q.ldc + n, &out, 16);
+			}
+			__builtin_amdgcn_sched_barrier(0);
+		}
+	}
+	if (partial == nullptr) return;
+	__syncthreads();  // (the weights are read)
+	float* all = reinterpret_cast<float*>(weights);
+	static_assert(16u * KT * 32u * 4u <= sizeof(weights), "");
+	if (i < 8u)
+#pragma unroll
+		for (uint32_t kk = 0; kk < KT; ++kk) all[wave * KT * 32u + kk * 32u + g * 8u + i] = sums[kk];
+	__syncthreads();
+	if (threadIdx.x < min(KT * 32u, q.k)) {
+		float sum = 0.f;
+#pragma unroll
+		for (uint32_t w = 0; w < 16u; ++w) sum += all[w * KT * 32u + threadIdx.x];
+		partial[(uint64_t)blockIdx.x * q.k + threadIdx.x] = sum;
+	}
+}
+
 // -------------------------------------------------------------------------------------------------------------------------------------
 // dz = dy * act'(z), and its column sums
 // -------------------------------------------------------------------------------------------------------------------------------------
@@ -619,10 +723,7 @@ __global__ void __launch_bounds__(256) slope_kernel(uint32_t n_rows, uint32_t wi
 			if (kind != N2_ACTIVATION_NONE) pre = n2_load_vec(z + row * ld_z + column, n);
 #pragma unroll
 			for (uint32_t i = 0; i < VEC; ++i) {
-				float v = (float)g.v[i];
-				if (kind == N2_ACTIVATION_RELU) v = (float)pre.v[i] > 0.f ? v : 0.f;
-				else if (kind != N2_ACTIVATION_NONE) v *= activation_slope((float)pre.v[i], kind);
-				v = i < n ? v : 0.f;
+				const float v = i < n ? slope_times((float)g.v[i], (float)pre.v[i], kind) : 0.f;
 				sum[i] += v;
 				out.v[i] = (T)v;
 			}
@@ -771,8 +872,8 @@ N2_API int n2_linear_forward(n2_stream_t stream, n2_dtype dtype, n2_activation a
 			auto launch = [&](auto kt, auto nt) {
 				constexpr uint32_t KT = decltype(kt)::value, NT = decltype(nt)::value;
 				const dim3 grid(n2_linear_stream_blocks(n_rows, KT * NT * 1024u));
-				if (d_residual != nullptr) stream_rows_kernel<T, KT, NT, true, true><<<grid, dim3(1024), 0, n2_stream(stream)>>>(q);
-				else stream_rows_kernel<T, KT, NT, false, true><<<grid, dim3(1024), 0, n2_stream(stream)>>>(q);
+				if (d_residual != nullptr) stream_rows_kernel<T, KT, NT, true><<<grid, dim3(1024), 0, n2_stream(stream)>>>(q);
+				else stream_rows_kernel<T, KT, NT, false><<<grid, dim3(1024), 0, n2_stream(stream)>>>(q);
 			};
 			with_narrow(in_width, out_width, launch);
 			N2_LAUNCH_CHECK();
@@ -833,7 +934,16 @@ N2_API int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation 
 		const bool products = d_dL_dinput != nullptr || dw != nullptr, aligned = reinterpret_cast<uintptr_t>(d_dL_doutput) % 16 == 0 && dL_doutput_stride % 8 == 0 && out_width % 8 == 0;
 		const bool writes = products && (activation != N2_ACTIVATION_NONE || !aligned);
 		Operand dz = {d_dL_doutput, dL_doutput_stride, false};
-		if (n_rows > 0 && (writes || db != nullptr)) {
+		uint32_t sum_rows = n_rows > 0 ? p.sum_blocks : 0u;
+		const bool has_x = d_dL_dinput != nullptr && n_rows > 0;
+		// Narrow layers of many rows: dx by stream_backward_kernel.  It forms dz and sums its columns on the way where dz need not be stored; with the
+		// store as well it took what two launches take (2^18 x 256 x 256 with ReLU 136 us for 73 and 62, 100 000 x 256 x 256 3 us more).  Where both
+		// products fit one launch (product_pair_kernel) that is the faster way from a stored dz (50 000 x 200 x 136 45 us for 49).
+		const bool small = p.input.tile == 64 && p.weights.tile == 64, forms_dz = activation == N2_ACTIVATION_NONE || dw == nullptr;
+		const bool streams = has_x && n2_linear_streams(n_rows, in_width, out_width) && (forms_dz || !small) && rows_of_vectors(d_dL_doutput, dL_doutput_stride, out_width) &&
+		                     rows_of_vectors(d_pre_activation, pre_stride, out_width) && rows_of_vectors(d_weights, in_width, in_width) && rows_of_vectors(d_dL_dinput, dL_dinput_stride, in_width);
+		const bool forms = streams && forms_dz;
+		if (!forms && n_rows > 0 && (writes || db != nullptr)) {
 			if (writes) dz = {ws, p.ld_dz, true};
 			auto launch = [&](auto lanes) {
 				constexpr uint32_t LANES = decltype(lanes)::value;
@@ -846,9 +956,21 @@ N2_API int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation 
 			else launch(std::integral_constant<uint32_t, 64>{});
 			N2_LAUNCH_CHECK();
 		}
+		if (streams) {
+			Product q = {};
+			q.a = dz, q.b = {d_weights, in_width, false};
+			q.m = n_rows, q.n = in_width, q.k = out_width;
+			q.c = d_dL_dinput, q.ldc = dL_dinput_stride, q.activation = activation;
+			with_narrow(out_width, in_width, [&](auto kt, auto nt) {
+				constexpr uint32_t KT = decltype(kt)::value, NT = decltype(nt)::value;
+				const uint32_t blocks = n2_linear_stream_blocks(n_rows, KT * NT * 1024u);
+				if (forms) sum_rows = blocks;
+				stream_backward_kernel<T, KT, NT><<<dim3(blocks), dim3(1024), 0, s>>>(q, forms ? static_cast<const T*>(d_pre_activation) : nullptr, pre_stride, forms && db != nullptr ? sums : nullptr);
+			});
+			N2_LAUNCH_CHECK();
+		}
 		Product x = {}, w = {};
-		const bool has_x = d_dL_dinput != nullptr && n_rows > 0;
-		if (has_x) {
+		if (has_x && !streams) {
 			x.a = dz, x.b = {d_weights, in_width, false};
 			x.m = n_rows, x.n = in_width, x.k = out_width;
 			x.c = d_dL_dinput, x.ldc = dL_dinput_stride;
@@ -862,28 +984,20 @@ N2_API int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation 
 			plan_product(w, p.weights, partial + p.input_partial);
 		}
 		const bool async = async_product<true, false>(x);
-		if (has_x && dw != nullptr && p.input.tile == 64 && p.weights.tile == 64 && async == async_product<false, false>(w) && blocks_of(x) + blocks_of(w) <= 0xFFFFFFFFull / 512u) {
+		if (has_x && !streams && dw != nullptr && small && async == async_product<false, false>(w) && blocks_of(x) + blocks_of(w) <= 0xFFFFFFFFull / 512u) {
 			const dim3 grid((uint32_t)(blocks_of(x) + blocks_of(w)));
 			if (async) product_pair_kernel<T, true><<<grid, dim3(256), 0, s>>>(x, w, (uint32_t)blocks_of(x));
 			else product_pair_kernel<T, false><<<grid, dim3(256), 0, s>>>(x, w, (uint32_t)blocks_of(x));
 			N2_LAUNCH_CHECK();
 		} else {
-			if (has_x && n2_linear_streams(n_rows, in_width, out_width) && async && x.k % 8 == 0 && rows_of_vectors(d_dL_dinput, dL_dinput_stride, in_width)) {
-				with_narrow(out_width, in_width, [&](auto kt, auto nt) {
-					constexpr uint32_t KT = decltype(kt)::value, NT = decltype(nt)::value;
-					stream_rows_kernel<T, KT, NT, false, false><<<dim3(n2_linear_stream_blocks(n_rows, KT * NT * 1024u)), dim3(1024), 0, s>>>(x);
-				});
-				N2_LAUNCH_CHECK();
-				x.partial = nullptr;
-			} else if (has_x) {
+			if (has_x && !streams)
 				if (const int rc = launch_product<T, true, false, STORE>(s, x, p.input.tile)) return rc;
-			}
 			if (dw != nullptr)
 				if (const int rc = launch_product<T, false, false, GRADIENT>(s, w, p.weights.tile)) return rc;
 		}
 		const uint32_t blocks_x = join_blocks(x), blocks_w = join_blocks(w), blocks_b = db != nullptr ? n2_ceil_div(out_width, 16u) : 0u;
 		if (blocks_x + blocks_w + blocks_b > 0) {
-			join_backward_kernel<T><<<dim3(blocks_x + blocks_w + blocks_b), dim3(256), 0, s>>>(x, blocks_x, w, blocks_w, sums, n_rows > 0 ? p.sum_blocks : 0u, out_width, static_cast<T*>(db), accumulate);
+			join_backward_kernel<T><<<dim3(blocks_x + blocks_w + blocks_b), dim3(256), 0, s>>>(x, blocks_x, w, blocks_w, sums, sum_rows, out_width, static_cast<T*>(db), accumulate);
 			N2_LAUNCH_CHECK();
 		}
 		return N2_OK;

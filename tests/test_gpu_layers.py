@@ -130,6 +130,33 @@ def test_linear_forward_of_many_rows(n, i, o, residual, kind, dtype):
 
 
 @pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("n,i,o,kind,mode", [(49152, 256, 256, "ReLU", 1), (49155, 64, 64, "SiLU", 2), (50001, 200, 136, "GELU", 1), (60000, 8, 8, "None", 1), (50000, 72, 256, "None", 2), (70001, 24, 128, "ReLU", 1),
+                                             (49200, 256, 64, "SiLU", 0), (49153, 36, 68, "GELU", 1), (49160, 33, 64, "ReLU", 1)])
+def test_linear_backward_of_many_rows(n, i, o, kind, mode, dtype):
+    """Narrow layers of many rows form dz, its column sums and dx in one pass; the parts on their own, the last rows ragged."""
+    gen = torch.Generator().manual_seed(n + o)
+    op, w, b = _linear(gen, i, o, kind, bias=True, dtype=dtype)
+    x, dy = _rows(gen, n, i, dtype), _rows(gen, n, o, dtype, 8, 8, scale=0.02)
+    z = _rows(gen, n, o, dtype, 8, 0) if kind != "None" else None
+    out, check = _canvas(n, i, dtype, 8, 8)
+    before = torch.randn(op.n_params(), generator=gen).to(dtype).cuda()
+    op._grads.copy_(before)
+    op.backward(x, z, dy, mode=mode, out=out)
+    check()
+    e = ref.linear_backward(x, w, z, dy, kind)
+    ref.within(out, *e["dx"], "dx")
+    old = before.double() * (mode == 2)
+    if mode == 0:
+        assert torch.equal(op._grads, before)
+    else:
+        for name, got, was in (("dw", op._grads[:o * i].view(o, i), old[:o * i].view(o, i)), ("db", op._grads[o * i:], old[o * i:])):
+            ref.within(got, e[name][0] + was, e[name][1] + ref.U32 * (e[name][0].abs() + was.abs()), name)
+    first = op._grads.clone()
+    op._grads.copy_(before)
+    assert torch.equal(op.backward(x, z, dy, mode=mode), out) and torch.equal(op._grads, first)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
 def test_linear_of_no_rows(dtype):
     from neus2_amd.capi import GRAD_ACCUMULATE
     gen = torch.Generator().manual_seed(1)
