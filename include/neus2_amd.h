@@ -917,10 +917,11 @@ void n2_snapshot_close(n2_snapshot_t* snapshot);
  * Rows: a matrix of n rows and c columns has element (i, j) at i * stride + j (elements, stride >= c): one row per
  * sample, unlike the SoA matrices above.  Rows need no alignment beyond their type's.  Sums, statistics and norms are
  * held in fp32 or more whatever the type; what is stored is rounded once.
- * No call touches what lies behind the last row or between a row's end and the next row.
+ * No call writes behind the last row or between a row's end and the next row, and no value that stands there matters.
  * An output may be the same rows as the residual (d_output == d_residual with equal strides, also for d_dL_dskip and
  * d_dL_dinput); any other overlap of what is written with what is read or written is refused.
- * Every sum is formed in an order that follows from the sizes alone: two calls on the same inputs give the same bits.
+ * Every sum is formed in an order that follows from sizes, strides and alignment alone: two calls on the same memory give
+ * the same bits.  What the calls enqueue may be captured; n2_gradients_create waits on the host and refuses a captured stream.
  * The workspaces are read only behind what the same call has written; calls that may run at the same time (also two
  * captured graphs) need workspaces of their own.
  * ---------------------------------------------------------------------- */
@@ -998,7 +999,8 @@ typedef struct n2_gradient_tensor {
 	uint32_t dtype;          /* n2_dtype */
 } n2_gradient_tensor;
 /* The tensors must not overlap each other.  d_table: n2_gradients_table_bytes of device memory, 16-byte aligned, the
- * object's until it is destroyed; the call fills it and waits for that on the host (not under stream capture). */
+ * object's until it is destroyed and the work of its calls is done; the call fills it and waits for that on the host.
+ * The sums of a call are joined in d_workspace, so calls that may run at the same time need one each. */
 uint64_t n2_gradients_table_bytes(uint32_t n_tensors, const n2_gradient_tensor* tensors);
 int n2_gradients_create(n2_stream_t stream, uint32_t n_tensors, const n2_gradient_tensor* tensors, void* d_table, uint64_t table_bytes,
                         n2_gradients_t** out);

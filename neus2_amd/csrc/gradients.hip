@@ -132,7 +132,7 @@ uint64_t piece_values(uint64_t all_bytes, uint32_t dtype) {
 }
 uint64_t all_bytes_of(uint32_t n_tensors, const n2_gradient_tensor* tensors) {
 	uint64_t bytes = 0;
-	for (uint32_t i = 0; i < n_tensors; ++i) bytes += std::min<uint64_t>(tensors[i].n, 1ull << 44) * n2_dtype_bytes(tensors[i].dtype);
+	for (uint32_t i = 0; i < n_tensors; ++i) bytes += std::min<uint64_t>(tensors[i].n, 1ull << 38) * n2_dtype_bytes(tensors[i].dtype);
 	return bytes;
 }
 
@@ -158,6 +158,7 @@ N2_API int n2_gradients_create(n2_stream_t stream, uint32_t n_tensors, const n2_
 	N2_REQUIRE(out != nullptr, "n2_gradients_create: out is null");
 	*out = nullptr;
 	N2_REQUIRE(n_tensors == 0 || tensors != nullptr, "n2_gradients_create: null tensors");
+	N2_REQUIRE(n_tensors < (1u << 24), "n2_gradients_create: %u tensors", n_tensors);
 	try {
 		struct Range { uintptr_t begin, end; };
 		std::vector<Range> ranges;
@@ -169,7 +170,7 @@ N2_API int n2_gradients_create(n2_stream_t stream, uint32_t n_tensors, const n2_
 			if (t.n == 0) continue;
 			const uint64_t bytes = n2_dtype_bytes(t.dtype);
 			N2_REQUIRE(t.d_gradients && t.d_out, "n2_gradients_create: tensor %u is null", i);
-			N2_REQUIRE(t.n < (1ull << 44), "n2_gradients_create: tensor %u has %llu values", i, (unsigned long long)t.n);
+			N2_REQUIRE(t.n < (1ull << 38), "n2_gradients_create: tensor %u has %llu values", i, (unsigned long long)t.n);
 			N2_REQUIRE((reinterpret_cast<uintptr_t>(t.d_gradients) | reinterpret_cast<uintptr_t>(t.d_out)) % bytes == 0, "n2_gradients_create: tensor %u is not aligned to its type", i);
 			const uintptr_t in = reinterpret_cast<uintptr_t>(t.d_gradients), to = reinterpret_cast<uintptr_t>(t.d_out);
 			ranges.push_back({in, in + t.n * bytes});
@@ -184,6 +185,11 @@ N2_API int n2_gradients_create(n2_stream_t stream, uint32_t n_tensors, const n2_
 		N2_REQUIRE(pieces.size() < (1ull << 31), "n2_gradients_create: too many values");
 		N2_REQUIRE(d_table && reinterpret_cast<uintptr_t>(d_table) % 16 == 0 && table_bytes >= needed, "n2_gradients_create: needs a 16-byte aligned table of %llu bytes, got %llu",
 		           (unsigned long long)needed, (unsigned long long)table_bytes);
+		if (!pieces.empty()) {
+			hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+			N2_HIP(hipStreamIsCapturing(n2_stream(stream), &capturing));
+			N2_REQUIRE(capturing == hipStreamCaptureStatusNone, "n2_gradients_create: the stream is being captured");
+		}
 		n2_gradients* g = new n2_gradients();
 		g->table = static_cast<const Piece*>(d_table);
 		g->n_pieces = (uint32_t)pieces.size();

@@ -397,20 +397,25 @@ __device__ __forceinline__ void product_async(const Product& q, uint32_t block, 
 		for (uint32_t i = 0; i < b_tile.LOADS; ++i) b_tile.load(tile_b0, i, left);
 		a_tile.advance(), b_tile.advance();
 	}
+	// a stage is there once every wave's loads into LDS have arrived; the one before it has been read by then
+	auto arrived = []() __attribute__((always_inline)) {
+		__builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+		__syncthreads();
+	};
 	// (stages come in pairs: a branch out between the two would have the sums in other registers there)
 	for (uint32_t pair = 0; pair < stages / 2u; ++pair) {
 		left -= BK;
-		__syncthreads();
+		arrived();
 		product_stage<T, A_KC, B_KC, BM, BN, RUN, THREADS>(tile_a0, tile_b0, tile_a1, tile_b1, left, a_read, b_read, a_tile, b_tile, acc);
 		left -= min(left, BK);
-		__syncthreads();
+		arrived();
 		product_stage<T, A_KC, B_KC, BM, BN, RUN, THREADS>(tile_a1, tile_b1, tile_a0, tile_b0, left, a_read, b_read, a_tile, b_tile, acc);
 	}
 	if (stages % 2u != 0u) {
-		__syncthreads();
+		arrived();
 		product_stage<T, A_KC, B_KC, BM, BN, RUN, THREADS>(tile_a0, tile_b0, tile_a1, tile_b1, 0u, a_read, b_read, a_tile, b_tile, acc);
 	}
-	__syncthreads();
+	arrived();
 	finish_all<T, EPI, OUT, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a0));
 }
 

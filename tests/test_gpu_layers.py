@@ -568,3 +568,84 @@ def test_two_streams_at_once():
     for k, (op, *_) in enumerate(pairs):
         assert torch.equal(op._grads, alone[k][1])
         assert all(torch.equal(t, alone[k][0]) for t in together[k::2])
+
+
+def test_rows_beyond_32_bits():
+    """More than 2^32 values in a matrix: the last rows are found by every pass (all others are zero, or checked by a sample)."""
+    n, i, last = 17_000_000, 256, 50
+    gen = torch.Generator().manual_seed(21)
+    x = torch.zeros(n, i, dtype=torch.float16, device="cuda")
+    x[-last:] = torch.randn(last, i, generator=gen).half().cuda()
+    for o in (8, 264):  # with the weights in LDS, and in tiles
+        op, w, b = _linear(gen, i, o, "None", bias=True, dtype=torch.float16)
+        y = op.forward(x)[0]
+        ye, _, dy_, _ = ref.linear_forward(x[-last:], w, b, None, "None")
+        ref.within(y[-last:], ye, dy_, "y")
+        ref.within(y[:1000], b.double().expand(1000, o), 0.0, "y of zeros")
+        dy = torch.randn(1000, o, generator=gen).half().cuda().repeat(n // 1000, 1)
+        dx = op.backward(x, None, dy)
+        e = ref.linear_backward(x[-last:], w, None, dy[-last:], "None")
+        ref.within(dx[-last:], *e["dx"], "dx")
+        ref.within(dx[n // 2 - 500:n // 2 + 500], *ref.linear_backward(x[:1000], w, None, dy[n // 2 - 500:n // 2 + 500], "None")["dx"], "dx of a sample")
+        ref.within(op._grads[:o * i].view(o, i), *e["dw"], "dw")
+        del y, dy, dx
+    op, scale, shift = _norm(gen, i, torch.float16, torch.float16)
+    y, (mean, rstd) = op.forward(x, want_ctx=True)
+    ref.within(y[-last:], *ref.norm_forward(x[-last:], scale, shift, 1e-5)[0], "norm")
+    ref.within(y[:1000], shift.double().expand(1000, i), 0.0, "norm of zeros")
+    dy = torch.zeros_like(x)
+    dy[-last:] = torch.randn(last, i, generator=gen).half().cuda()
+    dx = op.backward((mean, rstd), x, dy, dL_dskip=x)
+    e = ref.norm_backward(x[-last:], mean[-last:], rstd[-last:], scale, dy[-last:], x[-last:])
+    ref.within(dx[-last:], *e["dx"], "norm dx")
+    ref.within(op._grads[:i], *e["dscale"], "dscale")
+    assert not bool(dx[:-last].any())
+    del y, dx, dy
+
+
+def test_clip_of_one_tensor_beyond_32_bits():
+    from neus2_amd.layers import GradientClip
+    n = (1 << 32) + 12345
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g[-3:] = torch.tensor([3.0, 0.0, 4.0])
+    clip = GradientClip([g])
+    assert float(clip.clip(1.0)) == 5.0
+    assert [float(v) for v in g[-3:]] == pytest.approx([0.6, 0.0, 0.8], rel=2 ** -8) and not bool(g[:-3].any())
+
+
+def test_a_clip_is_not_made_under_capture():
+    from neus2_amd.capi import N2Error
+    from neus2_amd.layers import GradientClip
+    g = torch.ones(100, device="cuda")
+    graph, refused = torch.cuda.CUDAGraph(), []
+    with torch.cuda.graph(graph):
+        try:
+            GradientClip([g])
+        except N2Error as e:
+            refused.append(str(e))
+        g.mul_(2.0)
+    assert len(refused) == 1 and "captured" in refused[0]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(g[0]) == 2.0 and float(GradientClip([g]).norm()) == 20.0
+
+
+def test_layers_refuse_other_types_shapes_and_orders():
+    from neus2_amd.capi import N2Error
+    from neus2_amd.layers import GradientClip, LayerNorm, Linear
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16, device="cuda")
+    lin, norm = Linear(8, 4, activation="ReLU"), LayerNorm(8)
+    for call in (lambda: lin.set_params(h(35)), lambda: lin.set_params(h(36).float()), lambda: lin.set_params(h(72)[::2]), lambda: norm.set_params(h(15)), lambda: norm.set_params(h(16).float())):
+        with pytest.raises(N2Error):
+            call()
+    lin.set_params(h(36)), norm.set_params(h(16))
+    x, y = h(5, 8), h(5, 4)
+    ctx = norm.forward(x, want_ctx=True)[1]
+    for call in (lambda: lin.forward(h(5, 7)), lambda: lin.forward(x.float()), lambda: lin.forward(h(8, 5).t()), lambda: lin.forward(x, residual=h(4, 4)), lambda: lin.forward(x, out=h(5, 5)),
+                 lambda: lin.forward(x, residual=h(1, 4).expand(5, 4)), lambda: lin.forward(x.cpu()), lambda: lin.backward(x, None, y), lambda: lin.backward(x, y, y),  # (no gradients were set)
+                 lambda: lin.forward(x, out=x[:, :4]), lambda: norm.forward(x, out=x), lambda: norm.backward(None, x, x), lambda: norm.backward(ctx, x, x), lambda: norm.forward(h(5, 9)),
+                 lambda: norm.backward((ctx[0][:4], ctx[1]), x, x, mode=0), lambda: norm.backward(ctx, x, x, dL_dskip=x, want_input_grad=False, mode=0),
+                 lambda: GradientClip([h(4, 4).t()[:2]]), lambda: GradientClip([x, x]), lambda: GradientClip([x], out=[y]), lambda: GradientClip([x, y], out=[x]),
+                 lambda: GradientClip([torch.zeros(3, dtype=torch.int32, device="cuda")]), lambda: GradientClip([x[:, ::2]])):
+        with pytest.raises(N2Error):
+            call()

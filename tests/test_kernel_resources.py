@@ -25,3 +25,11 @@ def test_the_lattices_fine_levels_have_their_waves(tmp_path):
     found = {k: v for k, v in resources("lattice.hip", tmp_path).items() if "lattice_fine_kernel" in k}
     assert sorted(v[0] for v in found.values()) == [5, 6]
     assert all(registers <= 80 and spilled == 0 for _, registers, spilled in found.values())
+
+
+@pytest.mark.skipif(not os.path.exists(build.HIPCC), reason="needs hipcc")
+def test_the_linear_layers_sums_stay_in_registers(tmp_path):
+    """A product's tile is most of a wave's registers: a spilled one goes to memory in every stage."""
+    found = resources("linear.hip", tmp_path)
+    assert sum("product_kernel" in k for k in found) >= 36 and sum("stream_" in k for k in found) >= 54
+    assert not [k for k, v in found.items() if v[2] != 0]
