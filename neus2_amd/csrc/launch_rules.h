@@ -291,6 +291,14 @@ static inline uint32_t n2_linear_sum_blocks(uint32_t n_rows, uint32_t out_width)
 	return needed < most ? needed : most;
 }
 
+// Whether the pass that forms dz reads dy and z past the last-level cache: where that cannot hold what the whole backward pass goes over (dy, z, dz,
+// x and dx), dz, which both products read again, is what should stay there.  Backward in us, plain | streamed, ReLU: 2^18 x 256 x 256 (671 MB)
+// 216 | 195, 65 536 x 512 x 512 (336 MB) 155 | 138, 16 384 x 2048 x 2048 (336 MB) 295 | 280, 60 000 x 256 x 1024 (430 MB) 176 | 153, 2^18 x 128 x 128 (336 MB) 104 | 98,
+// 100 000 x 256 x 256 (256 MB) 95 | 93; 65 536 x 256 x 256 (168 MB) 65 | 72, 16 384 x 1024 x 1024 (168 MB) 107 | 111, 20 000 x 512 x 512 (102 MB) 68 | 70.
+static inline bool n2_linear_dz_streams(uint64_t n_rows, uint64_t in_width, uint64_t out_width) {
+	return 2u * n_rows * (3u * out_width + 2u * in_width) >= (240ull << 20);
+}
+
 // How C [m][n] of a sum over k is cut: square tiles to a workgroup, and where those are fewer than the CUs k is dealt out to several
 // workgroups for each, which leave fp32 sums that a second launch joins.
 struct N2LinearPlan {

@@ -36,6 +36,14 @@ __device__ __forceinline__ void n2_store_vec(T* __restrict__ p, const N2Vec<T>& 
 			if (i < valid) p[i] = r.v[i];
 	}
 }
+typedef n2_u32x4 n2_u32x4_anywhere __attribute__((aligned(2)));
+// n2_load_vec past the last-level cache (STREAM): for what is read once while something else is to stay there
+template <bool STREAM, typename T>
+__device__ __forceinline__ N2Vec<T> n2_load_vec_once(const T* __restrict__ p, uint32_t valid) {
+	if (STREAM && valid >= N2Vec<T>::SIZE) return __builtin_bit_cast(N2Vec<T>, (n2_u32x4)__builtin_nontemporal_load(reinterpret_cast<const n2_u32x4_anywhere*>(p)));
+	return n2_load_vec(p, valid);
+}
+
 // The vector at element `at` of a matrix whose last element is before `end`, zero from `valid` on.  Where a row's end leaves part of a vector
 // the rest is read with it as long as the matrix goes on; a lane that reads element by element holds up its whole wave.
 template <typename T>

@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(1024) stream_backward_kernel(Product q, const 
 // LANES lanes of eight values take a row (512 columns of it, where it is wider), rows as far apart as the launch has groups of lanes along
 // them.  dz (or null) goes into rows of ld_dz values, a multiple of eight, zero behind the width; partial (or null): one row of sums from
 // each workgroup.
-template <typename T, uint32_t LANES>
+template <typename T, uint32_t LANES, bool STREAM>
 __global__ void __launch_bounds__(256) slope_kernel(uint32_t n_rows, uint32_t width, const T* __restrict__ dy, uint64_t ld_dy, const T* __restrict__ z, uint64_t ld_z, int kind,
                                                     T* __restrict__ dz, uint64_t ld_dz, float* __restrict__ partial) {
 	constexpr uint32_t VEC = N2Vec<T>::SIZE, ROWS = 256u / LANES, COLUMNS = LANES * VEC;
@@ -723,9 +723,9 @@ __global__ void __launch_bounds__(256) slope_kernel(uint32_t n_rows, uint32_t wi
 	if (column < width) {
 #pragma unroll 4
 		for (uint64_t row = (uint64_t)blockIdx.y * ROWS + group; row < n_rows; row += (uint64_t)gridDim.y * ROWS) {
-			const N2Vec<T> g = n2_load_vec(dy + row * ld_dy + column, n);
+			const N2Vec<T> g = n2_load_vec_once<STREAM>(dy + row * ld_dy + column, n);
 			N2Vec<T> out = {}, pre = {};
-			if (kind != N2_ACTIVATION_NONE) pre = n2_load_vec(z + row * ld_z + column, n);
+			if (kind != N2_ACTIVATION_NONE) pre = n2_load_vec_once<STREAM>(z + row * ld_z + column, n);
 #pragma unroll
 			for (uint32_t i = 0; i < VEC; ++i) {
 				const float v = i < n ? slope_times((float)g.v[i], (float)pre.v[i], kind) : 0.f;
@@ -950,9 +950,12 @@ N2_API int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation 
 		const bool forms = streams && forms_dz;
 		if (!forms && n_rows > 0 && (writes || db != nullptr)) {
 			if (writes) dz = {ws, p.ld_dz, true};
+			const bool past_cache = writes && n2_linear_dz_streams(n_rows, in_width, out_width);
 			auto launch = [&](auto lanes) {
 				constexpr uint32_t LANES = decltype(lanes)::value;
-				slope_kernel<T, LANES><<<dim3(n2_ceil_div(out_width, LANES * 8u), p.sum_blocks), dim3(256), 0, s>>>(n_rows, out_width, static_cast<const T*>(d_dL_doutput), dL_doutput_stride,
+				if (past_cache) slope_kernel<T, LANES, true><<<dim3(n2_ceil_div(out_width, LANES * 8u), p.sum_blocks), dim3(256), 0, s>>>(n_rows, out_width, static_cast<const T*>(d_dL_doutput), dL_doutput_stride,
+					static_cast<const T*>(d_pre_activation), pre_stride, activation, writes ? reinterpret_cast<T*>(ws) : nullptr, p.ld_dz, db != nullptr ? sums : nullptr);
+				else slope_kernel<T, LANES, false><<<dim3(n2_ceil_div(out_width, LANES * 8u), p.sum_blocks), dim3(256), 0, s>>>(n_rows, out_width, static_cast<const T*>(d_dL_doutput), dL_doutput_stride,
 					static_cast<const T*>(d_pre_activation), pre_stride, activation, writes ? reinterpret_cast<T*>(ws) : nullptr, p.ld_dz, db != nullptr ? sums : nullptr);
 			};
 			if (out_width <= 64u) launch(std::integral_constant<uint32_t, 8>{});
