@@ -37,10 +37,10 @@ __device__ __forceinline__ float activation(float z, int kind) {
 	return z;
 }
 __device__ __forceinline__ float activation_slope(float z, int kind) {
-	if (kind == N2_ACTIVATION_RELU) return z > 0.f ? 1.f : 0.f;
 	if (kind == N2_ACTIVATION_SILU) {
-		const float s = __builtin_amdgcn_rcpf(1.f + fast_exp(-z));
-		return s * fmaf(z, 1.f - s, 1.f);
+		// s + z s (1 - s), s the logistic function, by u = exp(-|z|): 1 - s is formed without the difference, whose half step z would multiply
+		const float u = fast_exp(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.f + u), ur = u * r;
+		return fmaf(z * ur, r, z < 0.f ? ur : r);
 	}
 	if (kind == N2_ACTIVATION_GELU) {
 		const float gauss = fast_exp(-0.5f * z * z);
