@@ -203,6 +203,118 @@ def test_columns_behind_a_row_are_not_read():
         assert torch.equal(op.backward(*wide), dx) and torch.equal(op._grads, grads)
 
 
+@pytest.mark.parametrize("n,i,o", [(40, 72, 24), (300, 200, 136), (3000, 256, 256), (50000, 64, 128)])
+def test_linear_without_bias(n, i, o):
+    gen = torch.Generator().manual_seed(n + 1)
+    for dtype, kind in ((torch.float16, "ReLU"), (torch.bfloat16, "None")):
+        op, w, b = _linear(gen, i, o, kind, bias=False, dtype=dtype)
+        assert b is None and op.n_params() == i * o
+        x, dy = _rows(gen, n, i, dtype), _rows(gen, n, o, dtype, scale=0.1)
+        y, z = op.forward(x, want_pre_activation=True)
+        ye, _, error, _ = ref.linear_forward(x, w, None, None, kind)
+        ref.within(y, ye, error, "y")
+        dx = op.backward(x, z, dy)
+        e = ref.linear_backward(x, w, z, dy, kind)
+        ref.within(dx, *e["dx"], "dx")
+        ref.within(op._grads.view(o, i), *e["dw"], "dw")
+
+
+@pytest.mark.parametrize("n,i,o,extra,first,kind", [(100003, 256, 256, 0, 0, "ReLU"), (100003, 256, 257, 0, 0, "None"), (100010, 256, 256, 9, 1, "SiLU"), (33001, 512, 1024, 8, 8, "GELU"), (600001, 64, 64, 0, 0, "ReLU")])
+def test_linear_backward_of_more_than_the_cache_holds(n, i, o, extra, first, kind):
+    """dz formed by loads that pass by the last-level cache: whole vectors, odd widths, rows that start anywhere."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    make = lambda w, scale: (torch.randn(n, w + extra, generator=gen, device="cuda") * scale).half()[:, first:first + w]
+    op, w, b = _linear(torch.Generator().manual_seed(n), i, o, kind, bias=True, dtype=torch.float16)
+    x, z, dy = make(i, 1.0), make(o, 1.0) if kind != "None" else None, make(o, 0.01)
+    dx = op.backward(x, z, dy)
+    e = ref.linear_backward(x, w, z, dy, kind)
+    ref.within(dx, *e["dx"], "dx")
+    ref.within(op._grads[:o * i].view(o, i), *e["dw"], "dw")
+    ref.within(op._grads[o * i:], *e["db"], "db")
+    first_grads = op._grads.clone()
+    assert torch.equal(op.backward(x, z, dy), dx) and torch.equal(op._grads, first_grads)
+
+
+@pytest.mark.parametrize("n", [2, 40])
+def test_rows_a_long_way_apart(n):
+    """Strides beyond the 32-bit offsets of a tile's rows: 2^22 values and more from row to row."""
+    gen = torch.Generator().manual_seed(n + 5)
+    stride, i, o = (1 << 22) + 8, 72, 136
+    op, w, b = _linear(gen, i, o, "SiLU", bias=True, dtype=torch.bfloat16)
+    norm, *_ = _norm(gen, i, torch.bfloat16, torch.float32)
+    x, z, dy = (_rows(gen, n, c, torch.bfloat16) for c in (i, o, o))
+    whole = torch.full((n, stride), float("nan"), dtype=torch.bfloat16, device="cuda")
+    at = 0
+    wide = []
+    for t in (x, z, dy, x, z):  # (the last two: outputs)
+        view = whole[:, at:at + t.shape[1]]
+        at += t.shape[1] + 8
+        view.copy_(t)
+        wide.append(view)
+    far_x, far_z, far_dy, out_x, out_y = wide
+    y = op.forward(x, residual=dy)[0]
+    assert torch.equal(op.forward(far_x, residual=far_dy, out=out_y)[0], y)
+    dx = op.backward(x, z, dy)
+    grads = op._grads.clone()
+    assert torch.equal(op.backward(far_x, far_z, far_dy, out=out_x), dx)
+    e = ref.linear_backward(x, w, z, dy, "SiLU")
+    ref.within(out_x, *e["dx"], "dx")
+    ref.within(op._grads[:o * i].view(o, i), *e["dw"], "dw")
+    assert torch.equal(op._grads[o * i:], grads[o * i:])
+    h, ctx = norm.forward(x, want_ctx=True)
+    assert torch.equal(norm.forward(far_x, out=out_x)[0], h)
+    dh = norm.backward(ctx, x, h)
+    assert torch.equal(norm.backward(ctx, far_x, out_x, out=out_y[:, :i]), dh)
+    assert torch.equal(far_x, x) and torch.equal(far_z, z) and torch.equal(far_dy, dy)
+
+
+@pytest.mark.parametrize("n,i,o", [(1, 72, 40), (16, 72, 264), (50, 200, 136), (300, 328, 72), (3000, 264, 520), (49155, 72, 200), (49153, 256, 64), (50000, 264, 72)])
+def test_nothing_around_a_matrix_is_read(n, i, o):
+    """No numbers beside the columns and behind the last row of every operand, at strides of whole vectors."""
+    gen = torch.Generator().manual_seed(n + i + o)
+    op, w, b = _linear(gen, i, o, "ReLU", bias=True, dtype=torch.bfloat16)
+    x, z, dy, r = (_rows(gen, n, c, torch.bfloat16) for c in (i, o, o, o))
+    wide = []
+    for t in (x, z, dy, r):
+        m = torch.full((n + 70, t.shape[1] + 64), float("nan"), dtype=torch.bfloat16, device="cuda")
+        m[:n, :t.shape[1]] = t
+        wide.append(m[:n, :t.shape[1]])
+    assert torch.equal(op.forward(wide[0], residual=wide[3])[0], op.forward(x, residual=r)[0])
+    assert torch.equal(op.forward(wide[0])[0], op.forward(x)[0])
+    dx = op.backward(x, z, dy)
+    grads = op._grads.clone()
+    assert torch.equal(op.backward(*wide[:3]), dx) and torch.equal(op._grads, grads)
+    from neus2_amd.capi import GRAD_IGNORE
+    assert torch.equal(op.backward(*wide[:3], mode=GRAD_IGNORE), dx)
+    norm, *_ = _norm(gen, i, torch.bfloat16, torch.float32)
+    h, ctx = norm.forward(x, want_ctx=True)
+    assert torch.equal(norm.forward(wide[0])[0], h)
+    dh = norm.backward(ctx, x, x)
+    grads = norm._grads.clone()
+    assert torch.equal(norm.backward(ctx, wide[0], wide[0]), dh) and torch.equal(norm._grads, grads)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", HALVES)
+def test_activations_over_the_types_whole_range(kind, dtype):
+    """Every finite value of the type through the epilogue and through the slope, one layer of a single weight 1: no overflow on the way
+    turns a finite result into none."""
+    from neus2_amd.layers import Linear
+    values = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    values = values[torch.isfinite(values)].cuda()[:, None]
+    op = Linear(1, 1, activation=kind, bias=False, dtype=dtype)
+    one = torch.ones(1, dtype=dtype, device="cuda")
+    op.set_params(one, torch.zeros_like(one))
+    y, z = op.forward(values, want_pre_activation=True)
+    assert torch.equal(z.float(), values.float())
+    ye, _, error, _ = ref.linear_forward(values, one[:, None], None, None, kind)
+    ref.within(y, ye, error, "y")
+    dy = torch.full_like(values, 0.5)
+    dx = op.backward(values, z, dy, mode=0)
+    e = ref.linear_backward(values, one[:, None], values, dy, kind)
+    ref.within(dx, *e["dx"], "dx")
+
+
 def test_residual_in_place_and_columns_of_one_matrix():
     gen = torch.Generator().manual_seed(4)
     op, w, b = _linear(gen, 64, 64, "SiLU", bias=True, dtype=torch.float16)

@@ -18,6 +18,10 @@ extern "C" uint32_t xcd_order(uint32_t block, uint32_t blocks) { return n2_xcd_o
 extern "C" void tile_order(uint32_t tile, uint32_t tiles_m, uint32_t tiles_n, uint32_t* out) { n2_tile_order(tile, tiles_m, tiles_n, out[0], out[1]); }
 extern "C" uint32_t norm_forward_blocks(uint32_t rows, uint32_t per, uint32_t threads) { return n2_layer_norm_forward_blocks(rows, per, threads); }
 extern "C" uint32_t norm_backward_blocks(uint32_t rows, uint32_t per, uint32_t threads) { return n2_layer_norm_backward_blocks(rows, per, threads); }
+extern "C" uint32_t few_rows(uint32_t m) { return n2_linear_few_rows(m); }
+extern "C" uint32_t streams(uint32_t m, uint32_t n, uint32_t k) { return n2_linear_streams(m, n, k); }
+extern "C" uint32_t stream_blocks(uint32_t m, uint32_t lds) { return n2_linear_stream_blocks(m, lds); }
+extern "C" uint32_t dz_streams(uint64_t rows, uint64_t in, uint64_t out) { return n2_linear_dz_streams(rows, in, out); }
 extern "C" uint32_t sum_blocks(uint32_t rows, uint32_t width) { return n2_linear_sum_blocks(rows, width); }
 """
 
@@ -79,3 +83,16 @@ def test_blocks_of_the_passes_over_rows(rules):
         for width in (1, 64, 65, 256, 257, 4096, 65536):
             assert 1 <= rules.sum_blocks(rows, width) <= 1024
     assert rules.norm_forward_blocks(0, 4, 256) == rules.norm_backward_blocks(0, 4, 256) == 0 and rules.sum_blocks(0, 8) == 0
+
+
+def test_ways_change_where_their_measurements_cross(rules):
+    assert rules.few_rows(1) and rules.few_rows(16) and not rules.few_rows(17)
+    assert rules.streams(49152, 256, 256) and rules.streams(1 << 31, 1, 1)
+    assert not rules.streams(49151, 256, 256) and not rules.streams(1 << 20, 257, 256) and not rules.streams(1 << 20, 256, 257)
+    rules.dz_streams.argtypes = [C.c_uint64] * 3
+    assert rules.dz_streams(1 << 18, 256, 256) and rules.dz_streams((1 << 31) - 1, 65536, 65536)
+    assert not rules.dz_streams(65536, 256, 256) and not rules.dz_streams(1, 65536, 65536) and not rules.dz_streams(0, 1, 1)
+    for rows in (49152, 49153, 100000, (1 << 31) - 1):
+        for lds in (4096, 32768, 65536, 65537, 131072):
+            blocks = rules.stream_blocks(rows, lds)
+            assert 1 <= blocks <= (256 if lds > 65536 else 512) and (blocks - 1) * 256 < rows
