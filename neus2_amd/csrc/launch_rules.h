@@ -270,15 +270,19 @@ static inline N2GatherGrid n2_rows_of_blocks(uint32_t blocks, uint32_t threads) 
 	return {(x + N2_XCDS - 1u) / N2_XCDS * N2_XCDS, y};
 }
 
-// Workgroups of a layer norm's launch, each taking groups of rows as far apart as there are workgroups.  Backward, where each leaves two rows
-// of fp32 sums: at least four rows to one beyond the first 256.
+// Workgroups of a layer norm's launch, each taking groups of rows as far apart as there are workgroups: as many as are on the card at once.  Backward,
+// where each leaves two rows of fp32 sums that a second launch reads: beyond 256 of them only for four rows and two groups of rows to each.
+// GPU time in us, fp16: forward, 5000 x 4096 with 512, 1024 workgroups 19.2, 16.8 and 2000 x 16 384 with 256, 512, 1024 31.8, 34.5, 38.3; 262 144 x 256 with 1024,
+// 2048, 4096 52, 49, 47, 65 536 x 64 5.7, 6.0, 6.0.  Backward, 262 144 x 256 with 512, 1024, 1536 124, 86, 86, 65 536 x 64 13.6, 12.5, 16, 20 000 x 512 22, 19, 22; 2000 x 8192 with 256,
+// 500 39, 56; 1000 x 2048 with 256, 1000 16, 31, 3000 x 2048 with 375, 750, 1024 24.4, 26, 29, 5003 x 1001 with 625, 1024 18.7, 17.9; 30 000 x 16 with 235, 469, 938 11.1, 10.7, 12.8, 3000 x 256 with 94,
+// 188, 375 9.7, 8.6, 9.1.
 static inline uint32_t n2_layer_norm_forward_blocks(uint32_t n_rows, uint32_t rows_per_block, uint32_t threads) {
-	const uint32_t needed = n_rows / rows_per_block + (n_rows % rows_per_block != 0u), most = threads > 256u ? 512u : 2048u;
+	const uint32_t needed = n_rows / rows_per_block + (n_rows % rows_per_block != 0u), most = threads > 512u ? 256u : threads > 256u ? 1024u : 2048u;
 	return needed < most ? needed : most;
 }
 static inline uint32_t n2_layer_norm_backward_blocks(uint32_t n_rows, uint32_t rows_per_block, uint32_t threads) {
-	const uint32_t needed = n_rows / rows_per_block + (n_rows % rows_per_block != 0u), top = threads > 256u ? 512u : 1024u;
-	const uint32_t some = n_rows / 4u > 256u ? n_rows / 4u : 256u, most = some < top ? some : top;
+	const uint32_t needed = n_rows / rows_per_block + (n_rows % rows_per_block != 0u), top = threads > 512u ? 256u : threads > 256u ? 512u : 1024u;
+	const uint32_t worth = needed / 2u < n_rows / 4u ? needed / 2u : n_rows / 4u, some = worth > 256u ? worth : 256u, most = some < top ? some : top;
 	return needed < most ? needed : most;
 }
 

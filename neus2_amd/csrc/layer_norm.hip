@@ -1,21 +1,19 @@
 // Layer norm over rows of 1 to 16384 values, forward and backward.
 // What bounds it is memory: forward reads a row and writes one, backward reads two (three with a skip connection) and writes one.  A row
 // stays in the registers of the 8 to 1024 lanes that share it, so mean, variance (from the centred values: no cancellation) and result
-// come of one reading.
+// come of one reading.  fp16 on an MI355X: 262 144 x 256 forward 49 us (5.5 TB/s, some of it from the last-level cache; a large copy has 4.8), backward with
+// a skip connection 107 (5.0), 65 536 x 1024 47 and 115 (5.7, 4.7), 2000 x 16 384 32 and 95 (4.1, 2.8: one workgroup to a CU, and sums of 256 rows to join).
 #include "column_sums.h"
 
 #include <cmath>
 
 namespace {
 
-// LANES lanes share a row, each with CHUNKS vectors of it, LANES vectors apart.
+// LANES lanes share a row, each with CHUNKS vectors of it, LANES vectors apart, one row at a time: with few registers the other waves keep
+// memory busy.  (Four rows under way in a lane took, forward, 4.8 us for 3.3 at 300 x 256, 12 for 9.3 at 20 000 x 512, 52.6 for 49 at 262 144 x 256; two,
+// backward, 120 for 91 at 65 536 x 1024 and as long at 262 144 x 256.)
 template <uint32_t LANES>
 constexpr uint32_t threads_of() { return LANES > 256u ? LANES : 256u; }
-// Rows that a lane has under way at once, so that memory is kept busy: forward four vectors of them, backward, which reads two or three
-// matrices, two.
-template <uint32_t LANES, uint32_t CHUNKS, bool BACKWARD>
-constexpr uint32_t rows_at_once() { return BACKWARD ? (LANES > 64u ? 1u : 2u) : LANES > 512u ? 1u : LANES > 256u ? 2u : 4u; }
-
 // sums over the lanes of a row, in all of them
 template <uint32_t LANES, uint32_t N>
 __device__ __forceinline__ void row_sums(float (&v)[N], float (*shared)[N]) {
@@ -73,62 +71,47 @@ template <typename T, typename P, uint32_t LANES, uint32_t CHUNKS>
 __global__ void __launch_bounds__(threads_of<LANES>()) layer_norm_forward_kernel(uint32_t n_rows, uint32_t width, float epsilon, const P* __restrict__ scale, const P* __restrict__ shift,
                                                                                   const T* x, uint64_t x_stride, T* y, uint64_t y_stride, float* __restrict__ mean_out,
                                                                                   float* __restrict__ rstd_out) {
-	constexpr uint32_t VEC = N2Vec<T>::SIZE, ROWS = threads_of<LANES>() / LANES, R = rows_at_once<LANES, CHUNKS, false>();
-	__shared__ float shared[LANES > 64u ? threads_of<LANES>() / 64u : 1u][R];
+	constexpr uint32_t VEC = N2Vec<T>::SIZE, ROWS = threads_of<LANES>() / LANES;
+	__shared__ float shared[LANES > 64u ? threads_of<LANES>() / 64u : 1u][1];
 	const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
 	const float inv = 1.f / (float)width;
 	const uint64_t end = (uint64_t)(n_rows - 1u) * x_stride + width;
 	const Weights<P, LANES, CHUNKS, VEC> g(scale, width, lane), b(shift, width, lane);
 	// (the lanes of a workgroup's last rows stay for the barriers)
-	for (uint64_t first = (uint64_t)blockIdx.x * ROWS * R; first < n_rows; first += (uint64_t)gridDim.x * ROWS * R) {
-		N2Vec<T> in[R][CHUNKS];
-		float sum[R], mean[R];
+	for (uint64_t first = (uint64_t)blockIdx.x * ROWS; first < n_rows; first += (uint64_t)gridDim.x * ROWS) {
+		const uint64_t row = first + group;
+		N2Vec<T> in[CHUNKS];
+		float sum[1] = {0.f};
 #pragma unroll
-		for (uint32_t r = 0; r < R; ++r)
+		for (uint32_t c = 0; c < CHUNKS; ++c) {
+			const uint32_t at = (c * LANES + lane) * VEC;
+			in[c] = n2_load_row(x, row * x_stride + at, end, row < n_rows ? n2_left<T>(width, at) : 0u);
 #pragma unroll
-			for (uint32_t c = 0; c < CHUNKS; ++c) {
-				const uint64_t row = first + r * ROWS + group;
-				const uint32_t at = (c * LANES + lane) * VEC;
-				in[r][c] = n2_load_row(x, row * x_stride + at, end, row < n_rows ? n2_left<T>(width, at) : 0u);
-			}
-#pragma unroll
-		for (uint32_t r = 0; r < R; ++r) {
-			sum[r] = 0.f;
-#pragma unroll
-			for (uint32_t c = 0; c < CHUNKS; ++c)
-#pragma unroll
-				for (uint32_t i = 0; i < VEC; ++i) sum[r] += (float)in[r][c].v[i];
+			for (uint32_t i = 0; i < VEC; ++i) sum[0] += (float)in[c].v[i];
 		}
 		row_sums<LANES>(sum, shared);
+		const float mean = mean_of(sum[0], (float)width, inv);
+		sum[0] = 0.f;
 #pragma unroll
-		for (uint32_t r = 0; r < R; ++r) {
-			mean[r] = mean_of(sum[r], (float)width, inv);
-			sum[r] = 0.f;
+		for (uint32_t c = 0; c < CHUNKS; ++c)
 #pragma unroll
-			for (uint32_t c = 0; c < CHUNKS; ++c)
-#pragma unroll
-				for (uint32_t i = 0; i < VEC; ++i) {
-					const float d = (c * LANES + lane) * VEC + i < width ? (float)in[r][c].v[i] - mean[r] : 0.f;
-					sum[r] += d * d;
-				}
-		}
+			for (uint32_t i = 0; i < VEC; ++i) {
+				const float d = (c * LANES + lane) * VEC + i < width ? (float)in[c].v[i] - mean : 0.f;
+				sum[0] += d * d;
+			}
 		row_sums<LANES>(sum, shared);
+		const float rstd = rsqrtf(sum[0] * inv + epsilon);
+		if (row < n_rows && lane == 0u) {
+			if (mean_out != nullptr) mean_out[row] = mean;
+			if (rstd_out != nullptr) rstd_out[row] = rstd;
+		}
 #pragma unroll
-		for (uint32_t r = 0; r < R; ++r) {
-			const uint64_t row = first + r * ROWS + group;
-			const float rstd = rsqrtf(sum[r] * inv + epsilon);
-			if (row < n_rows && lane == 0u) {
-				if (mean_out != nullptr) mean_out[row] = mean[r];
-				if (rstd_out != nullptr) rstd_out[row] = rstd;
-			}
+		for (uint32_t c = 0; c < CHUNKS; ++c) {
+			const uint32_t at = (c * LANES + lane) * VEC;
+			N2Vec<T> out;
 #pragma unroll
-			for (uint32_t c = 0; c < CHUNKS; ++c) {
-				const uint32_t at = (c * LANES + lane) * VEC;
-				N2Vec<T> out;
-#pragma unroll
-				for (uint32_t i = 0; i < VEC; ++i) out.v[i] = (T)(((float)in[r][c].v[i] - mean[r]) * rstd * (float)g.v[c][i] + (float)b.v[c][i]);
-				n2_store_vec(y + row * y_stride + at, out, row < n_rows ? n2_left<T>(width, at) : 0u);
-			}
+			for (uint32_t i = 0; i < VEC; ++i) out.v[i] = (T)(((float)in[c].v[i] - mean) * rstd * (float)g.v[c][i] + (float)b.v[c][i]);
+			n2_store_vec(y + row * y_stride + at, out, row < n_rows ? n2_left<T>(width, at) : 0u);
 		}
 	}
 }
@@ -139,68 +122,55 @@ template <typename T, typename P, uint32_t LANES, uint32_t CHUNKS>
 __global__ void __launch_bounds__(threads_of<LANES>(), LANES <= 512u ? 4 : 1) layer_norm_backward_kernel(uint32_t n_rows, uint32_t width, const P* __restrict__ scale, const T* __restrict__ x, uint64_t x_stride,
                                                                                    const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ dy, uint64_t dy_stride,
                                                                                    const T* skip, uint64_t skip_stride, T* dx, uint64_t dx_stride, float* __restrict__ partial) {
-	constexpr uint32_t VEC = N2Vec<T>::SIZE, THREADS = threads_of<LANES>(), ROWS = THREADS / LANES, COLUMNS = LANES * CHUNKS * VEC, R = rows_at_once<LANES, CHUNKS, true>();
-	__shared__ float shared[LANES > 64u ? THREADS / 64u : 1u][2 * R];
+	constexpr uint32_t VEC = N2Vec<T>::SIZE, THREADS = threads_of<LANES>(), ROWS = THREADS / LANES, COLUMNS = LANES * CHUNKS * VEC;
+	__shared__ float shared[LANES > 64u ? THREADS / 64u : 1u][2];
 	const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
 	const float inv = 1.f / (float)width;
 	const uint64_t end_x = (uint64_t)(n_rows - 1u) * x_stride + width, end_dy = (uint64_t)(n_rows - 1u) * dy_stride + width, end_skip = (uint64_t)(n_rows - 1u) * skip_stride + width;
 	const Weights<P, LANES, CHUNKS, VEC> w(scale, width, lane);
 	float dscale[CHUNKS][VEC] = {}, dshift[CHUNKS][VEC] = {};
-	for (uint64_t first = (uint64_t)blockIdx.x * ROWS * R; first < n_rows; first += (uint64_t)gridDim.x * ROWS * R) {
-		N2Vec<T> in[R][CHUNKS], g[R][CHUNKS], add[R][CHUNKS];
-		float m[R], s[R], sum[2 * R];
+	for (uint64_t first = (uint64_t)blockIdx.x * ROWS; first < n_rows; first += (uint64_t)gridDim.x * ROWS) {
+		const uint64_t row = first + group;
+		const bool live = row < n_rows;
+		const float m = live ? mean[row] : 0.f, s = live ? rstd[row] : 0.f;
+		N2Vec<T> in[CHUNKS], g[CHUNKS], add[CHUNKS];
 #pragma unroll
-		for (uint32_t r = 0; r < R; ++r) {
-			const uint64_t row = first + r * ROWS + group;
-			const bool live = row < n_rows;
-			m[r] = live ? mean[row] : 0.f, s[r] = live ? rstd[row] : 0.f;
+		for (uint32_t c = 0; c < CHUNKS; ++c) {
+			const uint32_t at = (c * LANES + lane) * VEC, n = live ? n2_left<T>(width, at) : 0u;
+			in[c] = n2_load_row(x, row * x_stride + at, end_x, n);
+			g[c] = n2_load_row(dy, row * dy_stride + at, end_dy, n);
+			add[c] = N2Vec<T>{};
+			if (skip != nullptr) add[c] = n2_load_row(skip, row * skip_stride + at, end_skip, n);
+		}
+		float sum[2] = {0.f, 0.f};
 #pragma unroll
-			for (uint32_t c = 0; c < CHUNKS; ++c) {
-				const uint32_t at = (c * LANES + lane) * VEC, n = live ? n2_left<T>(width, at) : 0u;
-				in[r][c] = n2_load_row(x, row * x_stride + at, end_x, n);
-				g[r][c] = n2_load_row(dy, row * dy_stride + at, end_dy, n);
-				add[r][c] = N2Vec<T>{};
-				if (skip != nullptr) add[r][c] = n2_load_row(skip, row * skip_stride + at, end_skip, n);
+		for (uint32_t c = 0; c < CHUNKS; ++c)
+#pragma unroll
+			for (uint32_t i = 0; i < VEC; ++i) {
+				// (past the width, and for rows past the last, dy is zero and so is the scale)
+				const float xh = ((float)in[c].v[i] - m) * s, d = (float)g[c].v[i], h = d * (float)w.v[c][i];
+				dscale[c][i] += d * xh;
+				dshift[c][i] += d;
+				sum[0] += h;
+				sum[1] += h * xh;
 			}
-		}
-#pragma unroll
-		for (uint32_t r = 0; r < R; ++r) {
-			sum[2 * r] = sum[2 * r + 1] = 0.f;
-#pragma unroll
-			for (uint32_t c = 0; c < CHUNKS; ++c)
-#pragma unroll
-				for (uint32_t i = 0; i < VEC; ++i) {
-					// (past the width, and for rows past the last, dy is zero and so is the scale)
-					const float xh = ((float)in[r][c].v[i] - m[r]) * s[r], d = (float)g[r][c].v[i], h = d * (float)w.v[c][i];
-					dscale[c][i] += d * xh;
-					dshift[c][i] += d;
-					sum[2 * r] += h;
-					sum[2 * r + 1] += h * xh;
-				}
-		}
 		if (dx == nullptr) continue;
 		row_sums<LANES>(sum, shared);
 		// (the second half takes the rows' values from the registers they came in: kept as fp32 they would halve the waves)
 		if constexpr (LANES <= 256u)
 #pragma unroll
-			for (uint32_t r = 0; r < R; ++r)
+			for (uint32_t c = 0; c < CHUNKS; ++c) as_loaded(in[c]), as_loaded(g[c]);
+		const float a = sum[0] * inv, b = sum[1] * inv;
 #pragma unroll
-				for (uint32_t c = 0; c < CHUNKS; ++c) as_loaded(in[r][c]), as_loaded(g[r][c]);
+		for (uint32_t c = 0; c < CHUNKS; ++c) {
+			const uint32_t at = (c * LANES + lane) * VEC;
+			N2Vec<T> out;
 #pragma unroll
-		for (uint32_t r = 0; r < R; ++r) {
-			const uint64_t row = first + r * ROWS + group;
-			const float a = sum[2 * r] * inv, b = sum[2 * r + 1] * inv;
-#pragma unroll
-			for (uint32_t c = 0; c < CHUNKS; ++c) {
-				const uint32_t at = (c * LANES + lane) * VEC;
-				N2Vec<T> out;
-#pragma unroll
-				for (uint32_t i = 0; i < VEC; ++i) {
-					const float xh = ((float)in[r][c].v[i] - m[r]) * s[r], h = (float)g[r][c].v[i] * (float)w.v[c][i];
-					out.v[i] = (T)(s[r] * (h - a - xh * b) + (float)add[r][c].v[i]);
-				}
-				n2_store_vec(dx + row * dx_stride + at, out, row < n_rows ? n2_left<T>(width, at) : 0u);
+			for (uint32_t i = 0; i < VEC; ++i) {
+				const float xh = ((float)in[c].v[i] - m) * s, h = (float)g[c].v[i] * (float)w.v[c][i];
+				out.v[i] = (T)(s * (h - a - xh * b) + (float)add[c].v[i]);
 			}
+			n2_store_vec(dx + row * dx_stride + at, out, live ? n2_left<T>(width, at) : 0u);
 		}
 	}
 	if (partial == nullptr) return;
@@ -244,7 +214,9 @@ __global__ void __launch_bounds__(threads_of<LANES>(), LANES <= 512u ? 4 : 1) la
 struct Row {
 	uint32_t lanes, chunks;
 };
-// the fewest lanes that hold a row in one vector each, or in two or four where there are no more lanes to take
+// The fewest lanes that hold a row in one vector each, or in two or four where there are no more lanes to take.  With half the lanes and two vectors
+// in each, forward and backward took 59 and 361 us for 53 and 87 at 262 144 x 256, 10.5 and 43 for 8.8 and 18 at 5003 x 1001, 4.7 and 8.0 for 4.6 and 8.0 at
+// 1000 x 64 (fp16).
 Row row_of(uint32_t width, uint32_t vec) {
 	constexpr Row rows[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {128, 1}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
 	for (const Row& row : rows)
@@ -304,7 +276,7 @@ N2_API int n2_layer_norm_forward(n2_stream_t stream, n2_dtype dtype, n2_dtype we
 		using P = decltype(p);
 		with_row(row_of(width, N2Vec<T>::SIZE), [&](auto lanes, auto chunks) {
 			constexpr uint32_t LANES = decltype(lanes)::value, THREADS = threads_of<LANES>(), ROWS = THREADS / LANES;
-			const uint32_t blocks = n2_layer_norm_forward_blocks(n_rows, ROWS * rows_at_once<LANES, decltype(chunks)::value, false>(), THREADS);
+			const uint32_t blocks = n2_layer_norm_forward_blocks(n_rows, ROWS, THREADS);
 			layer_norm_forward_kernel<T, P, LANES, decltype(chunks)::value><<<dim3(blocks), dim3(THREADS), 0, n2_stream(stream)>>>(
 				n_rows, width, epsilon, static_cast<const P*>(d_scale), static_cast<const P*>(d_shift), static_cast<const T*>(d_input), input_stride, static_cast<T*>(d_output),
 				output_stride, d_mean, d_rstd);
@@ -319,7 +291,7 @@ N2_API uint64_t n2_layer_norm_workspace_bytes(n2_dtype dtype, uint32_t n_rows, u
 	uint64_t blocks = 0;
 	with_row(row_of(width, 16u / n2_dtype_bytes(dtype)), [&](auto lanes, auto chunks) {
 		constexpr uint32_t LANES = decltype(lanes)::value, THREADS = threads_of<LANES>();
-		blocks = n2_layer_norm_backward_blocks(n_rows, THREADS / LANES * rows_at_once<LANES, decltype(chunks)::value, true>(), THREADS);
+		blocks = n2_layer_norm_backward_blocks(n_rows, THREADS / LANES, THREADS);
 	});
 	return 8ull * width * blocks;
 }
@@ -359,7 +331,7 @@ N2_API int n2_layer_norm_backward(n2_stream_t stream, n2_dtype dtype, n2_dtype w
 			using P = decltype(p);
 			with_row(row_of(width, N2Vec<T>::SIZE), [&](auto lanes, auto chunks) {
 				constexpr uint32_t LANES = decltype(lanes)::value, THREADS = threads_of<LANES>(), ROWS = THREADS / LANES;
-				blocks = n2_layer_norm_backward_blocks(n_rows, ROWS * rows_at_once<LANES, decltype(chunks)::value, true>(), THREADS);
+				blocks = n2_layer_norm_backward_blocks(n_rows, ROWS, THREADS);
 				layer_norm_backward_kernel<T, P, LANES, decltype(chunks)::value><<<dim3(blocks), dim3(THREADS), 0, s>>>(
 					n_rows, width, static_cast<const P*>(d_scale), static_cast<const T*>(d_input), input_stride, d_mean, d_rstd, static_cast<const T*>(d_dL_doutput), dL_doutput_stride,
 					static_cast<const T*>(d_dL_dskip), dL_dskip_stride, static_cast<T*>(d_dL_dinput), dL_dinput_stride, weights ? static_cast<float*>(d_workspace) : nullptr);
