@@ -1,7 +1,9 @@
 // The norm over the gradients of many tensors and their clipping: two launches whatever the number of tensors.
 // The host cuts the tensors into pieces, about as many as there are workgroups at a time; a launch's workgroups take pieces in turn.  What
 // bounds both launches is memory: the first reads every gradient, the second reads and writes it, from the last pieces to the first, so that
-// what the first launch read last is still in the caches.
+// what the first launch read last is still in the caches.  On an MI355X the norm of 139 MB in 60 fp32 tensors takes 24 us (5.8 TB/s), of 800 MB
+// in two 142 (5.6); clipping 50 MB into other tensors 28 us for three times as many bytes (5.5), clipping in place where nothing is clipped
+// little more than the norm (26 and 146 us); four tensors of 1000 values 4.6 us, the launches.
 #include "layer_types.h"
 
 #include <algorithm>
@@ -20,7 +22,9 @@ struct Piece {
 static_assert(sizeof(Piece) == 32, "pieces are read by 16 bytes");
 
 constexpr uint32_t THREADS = 256, MAX_BLOCKS = N2_GRADIENTS_WORKSPACE_BYTES / sizeof(double);
-// Bytes to a piece: all pieces at once up to 32 MB, and long enough that a piece's entry in the table costs little beyond.
+// Bytes to a piece: 4 to 64 KB, so that up to 128 MB each of the 2048 workgroups has one piece; beyond, a piece's entry in the table costs little.  Clipping in
+// place with pieces up to 16, 32, 64 and 256 KB, us: 60 fp32 tensors, 139 MB, 27.4, 27.3, 26.4, 26.7; 8 fp16 tensors, 160 MB, 30.9, 29.9, 29.6, 29.8; 2 fp32
+// tensors, 800 MB, 150, 145, 146, 140.
 constexpr uint64_t PIECE_STEP = THREADS * 16, MOST_STEPS = 16;
 
 // Squares are summed in fp64: those of fp32 and bf16 leave fp32's range long before the values do.
@@ -40,7 +44,9 @@ __device__ __forceinline__ double squares<n2_f16>(const N2Vec<n2_f16>& v) {
 	return (double)s;
 }
 
-// f(vector, place, valid values) for a lane's vectors of a piece, four loads under way at a time
+// f(vector, place, valid values) for a lane's vectors of a piece, four loads under way at a time.  (The norm with two, four and eight, us: 40
+// fp16 tensors, 8 MB, 6.8, 6.8, 7.6; 60 fp32 tensors, 139 MB, 24.5, 23.7, 23.6; 4 fp32 tensors, 50 MB, 11.8, 12.8, 14.4: the loads of a piece's end are made
+// one by one.)
 template <typename T, typename F>
 __device__ __forceinline__ void each_vector(const Piece& p, F&& f) {
 	constexpr uint32_t VEC = N2Vec<T>::SIZE, STEP = THREADS * VEC;

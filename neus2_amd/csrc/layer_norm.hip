@@ -2,7 +2,7 @@
 // What bounds it is memory: forward reads a row and writes one, backward reads two (three with a skip connection) and writes one.  A row
 // stays in the registers of the 8 to 1024 lanes that share it, so mean, variance (from the centred values: no cancellation) and result
 // come of one reading.  fp16 on an MI355X: 262 144 x 256 forward 49 us (5.5 TB/s, some of it from the last-level cache; a large copy has 4.8), backward with
-// a skip connection 107 (5.0), 65 536 x 1024 47 and 115 (5.7, 4.7), 2000 x 16 384 32 and 95 (4.1, 2.8: one workgroup to a CU, and sums of 256 rows to join).
+// a skip connection 107 (5.0), 65 536 x 1024 47 and 115 (5.7, 4.7), 2000 x 16 384 32 and 98 (4.1, 2.7: one workgroup to a CU, and sums of 256 rows to join).
 #include "column_sums.h"
 
 #include <cmath>

@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(256) join_backward_kernel(Product x, uint32_t 
 	const uint32_t block = blockIdx.x;
 	if (block < blocks_x) join<T, STORE>(x, block);
 	else if (block - blocks_x < blocks_w) join<T, GRADIENT>(w, block - blocks_x);
-	else n2_column_sums_block<16, 1, 16>(sums, sum_rows, columns, block - blocks_x - blocks_w, [&](uint32_t column, float sum) { n2_store_sum(db + column, sum, accumulate); });
+	else n2_column_sums_block<16, 16>(sums, sum_rows, columns, block - blocks_x - blocks_w, [&](uint32_t column, float sum) { n2_store_sum(db + column, sum, accumulate); });
 }
 
 // A layer of up to sixteen rows: what it takes is the weights' way from memory, so sixteen columns of C go to a workgroup and its sixteen
