@@ -288,7 +288,9 @@ static inline uint32_t n2_layer_norm_backward_blocks(uint32_t n_rows, uint32_t r
 
 N2_HD inline uint32_t n2_ceil_div(uint64_t n, uint32_t by) { return (uint32_t)((n + by - 1u) / by); }
 
-// Workgroups along the rows of a linear layer's pass over dz, each leaving a row of column sums.
+// Workgroups along the rows of a linear layer's pass over dz, each leaving a row of column sums: about 1024 in all.  Backward with ReLU in us, up to
+// 512 | 1024 | 2048: 5003 x 320 x 257 25 | 24 | 27, 20 000 x 512 x 512 71 | 68 | 72, 100 000 x 256 x 256 96 | 86 | 91, 2^18 x 256 x 256 226 | 199 | 214, 16 384 x 2048 x 2048
+// 305 | 286 | 295.
 static inline uint32_t n2_linear_sum_blocks(uint32_t n_rows, uint32_t out_width) {
 	const uint32_t lanes = out_width <= 64u ? 8u : out_width <= 128u ? 16u : out_width <= 256u ? 32u : 64u, columns = n2_ceil_div(out_width, lanes * 8u);
 	const uint32_t most = 1024u / columns > 16u ? 1024u / columns : 16u, needed = n2_ceil_div(n_rows, 256u / lanes);
@@ -304,7 +306,11 @@ static inline bool n2_linear_dz_streams(uint64_t n_rows, uint64_t in_width, uint
 }
 
 // How C [m][n] of a sum over k is cut: square tiles to a workgroup, and where those are fewer than the CUs k is dealt out to several
-// workgroups for each, which leave fp32 sums that a second launch joins.
+// workgroups for each, which leave fp32 sums that a second launch joins.  GPU time in us, rows x in x out.  Forward with tiles of 64 | 128 | 256:
+// 4096 x 1024 x 1024 16 | 17 | 28, 20 000 x 512 x 512 23 | - | 26, 65 536 x 512 x 512 63 | 53 | 46, 16 384 x 2048 x 2048 220 | 154 | 116, 2^18 x 256 x 256 78 | 72 | 73.  dW's product (and the pass
+// over dz's column sums) with tile / splits: 16 384 x 2048 x 2048 256 / 4 145, 128 / 2 180; 65 536 x 512 x 512 256 / 64 72, 128 / 32 72; 2^18 x 256 x 256 128 / 128 101,
+// 256 / 128 107; 20 000 x 512 x 512 64 / 16 37, 128 / 32 39; 4096 x 1024 x 1024 64 / 4 33, 64 / 1 48.  Forward with small tiles and splits: 300 x 2048 x 2048 in two 16, in one 22;
+// 500 x 1000 x 1000 in two 10.4, in one 9 to 11.
 struct N2LinearPlan {
 	uint32_t tile, splits, k_per_split;
 };
@@ -322,7 +328,8 @@ static inline N2LinearPlan n2_linear_plan(uint32_t m, uint32_t n, uint32_t k) {
 	if (fits(128) && tiles_of(128) >= 1024) return {128, 1, k};
 	if (fits(256) && tiles_of(64) >= 1024 && k >= 4096) return split(256, 256u / tiles_of(256), k / 640u);
 	if (fits(128) && k >= 16384) return split(128, 512u / tiles_of(128), k / 640u);
-	// small tiles: what a launch takes in us, 3 and 0.45 for a stage of 64 (times as many as do not run at once), and what joining takes
+	// small tiles: what the launches take in us beyond the first's own, fitted to such times: 0.45 for a stage of 64 of k (times the turns of the
+	// 512 workgroups that run at once), and for joining 2, 0.05 for each split and the sums' way to memory and back at 3 TB/s
 	const uint32_t stages = n2_ceil_div(k, 64u);
 	const double tiles = (double)tiles_of(64);
 	uint32_t best = 1;
