@@ -315,6 +315,41 @@ def test_activations_over_the_types_whole_range(kind, dtype):
     ref.within(dx, *e["dx"], "dx")
 
 
+@pytest.mark.parametrize("n,i,o", [(3, 72, 40), (100, 256, 136), (5000, 64, 64), (50000, 64, 128)])
+def test_parameters_anywhere_in_a_larger_vector(n, i, o):
+    """A layer's parameters and gradients inside the vector of a whole network, at odd places: what stands beside them stays."""
+    from neus2_amd.layers import LayerNorm, Linear
+    gen = torch.Generator().manual_seed(n + 9)
+    dtype = torch.float16
+    lin, norm = Linear(i, o, activation="SiLU", dtype=dtype), LayerNorm(i, dtype=dtype)
+    at, after = 1, 1 + lin.n_params() + 2
+    size = after + norm.n_params() + 1
+    params = (torch.randn(size, generator=gen) * 0.1).to(dtype).cuda()
+    grads = torch.full((size,), 7.0, dtype=dtype, device="cuda")
+    lin.set_params(params[at:at + lin.n_params()], grads[at:at + lin.n_params()])
+    norm.set_params(params[after:after + norm.n_params()], grads[after:after + norm.n_params()])
+    x, dy = _rows(gen, n, i, dtype), _rows(gen, n, o, dtype, scale=0.05)
+    h, ctx = norm.forward(x, want_ctx=True)
+    y, z = lin.forward(h, want_pre_activation=True)
+    w, b = params[at:at + i * o].view(o, i), params[at + i * o:at + i * o + o]
+    scale, shift = params[after:after + i], params[after + i:after + 2 * i]
+    ref.within(h, *ref.norm_forward(x, scale, shift, 1e-5)[0], "h")
+    ye, _, error, _ = ref.linear_forward(h, w, b, None, "SiLU")
+    ref.within(y, ye, error, "y")
+    dh = lin.backward(h, z, dy)
+    e = ref.linear_backward(h, w, z, dy, "SiLU")
+    ref.within(dh, *e["dx"], "dh")
+    ref.within(grads[at:at + i * o].view(o, i), *e["dw"], "dw")
+    ref.within(grads[at + i * o:at + i * o + o], *e["db"], "db")
+    dx = norm.backward(ctx, x, dh)
+    e = ref.norm_backward(x, *ctx, scale, dh, None)
+    ref.within(dx, *e["dx"], "dx")
+    ref.within(grads[after:after + i], *e["dscale"], "dscale")
+    ref.within(grads[after + i:after + 2 * i], *e["dshift"], "dshift")
+    beside = torch.cat([grads[:at], grads[at + lin.n_params():after], grads[after + norm.n_params():]])
+    assert beside.numel() == 4 and bool((beside == 7.0).all())
+
+
 def test_residual_in_place_and_columns_of_one_matrix():
     gen = torch.Generator().manual_seed(4)
     op, w, b = _linear(gen, 64, 64, "SiLU", bias=True, dtype=torch.float16)
