@@ -98,26 +98,49 @@ __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
 	}
 }
 
-// the tile from index `first` and k0 on; what lies past the extent or past K is zero
+// A tile of an operand that may start at any element, on its way through registers: load() asks for the one from index `first` and k0 on, put()
+// writes it to LDS, zero past the extent and past K.  Every piece is one load of 16 bytes inside the matrix, moved back from its end where it
+// would go beyond, and only put(), a stage later, shifts and cuts it: nothing waits for a load before that.  (Loaded and put at once, element by
+// element at the rows' ends, a product took, forward, 56 us for 36 at 6836 x 3385 x 109, 70 for 60 at 139 043 x 255 x 111, 12 for 10.2 at 300 x 333 x 77,
+// backward with ReLU 45 for 40 at 12 783 x 279 x 216, 177 for 141 at 139 043 x 255 x 111.)
 template <typename T, bool KC, uint32_t R, uint32_t RUN, uint32_t THREADS>
-__device__ __forceinline__ void load_tile(uint4* __restrict__ lds, const Operand& o, uint32_t first, uint32_t extent, uint32_t k0, uint32_t k_end) {
-	const T* __restrict__ p = static_cast<const T*>(o.p);
-	constexpr uint32_t PIECES = R * BK / 8u, ROW = KC ? BK / 8u : R / 8u;
-#pragma unroll
-	for (uint32_t i = 0; i < PIECES / THREADS; ++i) {
+struct RegisterTile {
+	static constexpr uint32_t LOADS = R * BK / 8u / THREADS, ROW = KC ? BK / 8u : R / 8u;
+	const T* p;
+	uint64_t ld, end;  // the matrix is [p, p + end)
+	uint32_t first, extent;
+	uint4 v[LOADS];
+
+	__device__ __forceinline__ RegisterTile(const Operand& o, uint32_t from, uint32_t n, uint32_t k)
+		: p(static_cast<const T*>(o.p)), ld(o.ld), end(KC ? (uint64_t)(n - 1u) * o.ld + k : (uint64_t)(k - 1u) * o.ld + n), first(from), extent(n) {}
+	__device__ __forceinline__ uint64_t place_of(uint32_t i, uint32_t k0) const {
 		const uint32_t at = i * THREADS + threadIdx.x, row = at / ROW, piece = at % ROW;
-		uint32_t valid;
-		uint64_t from;
-		if constexpr (KC) {
-			valid = first + row < extent && k0 + piece * 8u < k_end ? min(k_end - (k0 + piece * 8u), 8u) : 0u;
-			from = (uint64_t)(first + row) * o.ld + k0 + piece * 8u;
-		} else {
-			valid = k0 + row < k_end && first + piece * 8u < extent ? min(extent - (first + piece * 8u), 8u) : 0u;
-			from = (uint64_t)(k0 + row) * o.ld + first + piece * 8u;
-		}
-		lds[place<KC, R, RUN>(row, piece)] = __builtin_bit_cast(uint4, n2_load_vec(p + from, valid));
+		return KC ? (uint64_t)(first + row) * ld + k0 + piece * 8u : (uint64_t)(k0 + row) * ld + first + piece * 8u;
 	}
-}
+	__device__ __forceinline__ void load(uint32_t k0) {
+		if (end < 8u) return;
+#pragma unroll
+		for (uint32_t i = 0; i < LOADS; ++i) __builtin_memcpy(&v[i], p + min(place_of(i, k0), end - 8u), 16);
+	}
+	__device__ __forceinline__ void put(uint4* __restrict__ lds, uint32_t k0, uint32_t k_end) {
+#pragma unroll
+		for (uint32_t i = 0; i < LOADS; ++i) {
+			const uint32_t at = i * THREADS + threadIdx.x, row = at / ROW, piece = at % ROW;
+			const uint32_t index = KC ? first + row : first + piece * 8u, k = KC ? k0 + piece * 8u : k0 + row;
+			const uint32_t valid = index < extent && k < k_end ? min(KC ? k_end - k : extent - index, 8u) : 0u;
+			if (end < 8u) {
+				v[i] = __builtin_bit_cast(uint4, n2_load_vec(p + (valid != 0u ? place_of(i, k0) : 0u), valid));
+			} else if (valid < 8u) {
+				typedef unsigned __int128 Bits;
+				const uint64_t from = place_of(i, k0), back = from + 8u > end ? from + 8u - end : 0u;
+				Bits bits = __builtin_bit_cast(Bits, v[i]);
+				bits = valid != 0u ? bits >> ((uint32_t)back * 16u) & ~(Bits)0 >> (128u - 16u * valid) : (Bits)0;
+				v[i] = __builtin_bit_cast(uint4, bits);
+			}
+			lds[place<KC, R, RUN>(row, piece)] = v[i];
+		}
+	}
+};
 
 // Reads operands of matrix instructions: 16 indices by 32 values of k, lane l holding index l % 16 and the eight values from 8 * (l / 16)
 // on.  The 16 indices are consecutive (RUN 4), or four runs of four, eight apart (RUN 8); number u begins at first + b_base(u).  The
@@ -285,10 +308,14 @@ __device__ __forceinline__ void product(const Product& q, uint32_t block, uint4*
 	const Fragments<A_KC, BM, 4u> a_read(wm);
 	const Fragments<B_KC, BN, RUN> b_read(wn);
 	f32x4 acc[S][U] = {};
+	RegisterTile<T, A_KC, BM, 4u, THREADS> a_tile(q.a, m0, q.m, q.k);
+	RegisterTile<T, B_KC, BN, RUN, THREADS> b_tile(q.b, n0, q.n, q.k);
+	if (k_begin < k_end) a_tile.load(k_begin), b_tile.load(k_begin);  // (of no rows there is nothing to load)
 	for (uint32_t k0 = k_begin; k0 < k_end; k0 += BK) {
-		load_tile<T, A_KC, BM, 4u, THREADS>(tile_a, q.a, m0, q.m, k0, k_end);
-		load_tile<T, B_KC, BN, RUN, THREADS>(tile_b, q.b, n0, q.n, k0, k_end);
+		a_tile.put(tile_a, k0, k_end);
+		b_tile.put(tile_b, k0, k_end);
 		__syncthreads();
+		a_tile.load(k0 + BK), b_tile.load(k0 + BK);  // (past the end of k: the matrix's last values, not used)
 #pragma unroll
 		for (uint32_t kk = 0; kk < BK / 32u; ++kk) {
 			s16x8 a[S], b[U];
@@ -306,7 +333,7 @@ __device__ __forceinline__ void product(const Product& q, uint32_t block, uint4*
 	finish_all<T, EPI, OUT, RUN>(q, m0 + wm, n0 + wn, split, acc, reinterpret_cast<float*>(tile_a));
 }
 
-// The tile of load_tile straight from memory into LDS (no register in between): 16 bytes from each lane's address go to the wave's place and
+// Such a tile straight from memory into LDS (no register in between): 16 bytes from each lane's address go to the wave's place and
 // 16 bytes times the lane, so a lane asks for the piece that belongs there.  Rows and pieces past the extent are the last ones once more; what
 // is computed from them is not stored.  Pieces past the end of k (a multiple of eight, for an operand contiguous in k) are zeros from g_zeros.
 __device__ const uint4 g_zeros = {0u, 0u, 0u, 0u};
