@@ -350,6 +350,26 @@ def test_parameters_anywhere_in_a_larger_vector(n, i, o):
     assert beside.numel() == 4 and bool((beside == 7.0).all())
 
 
+@pytest.mark.parametrize("n,i,o,extra,first", [(50001, 513, 510, 0, 0), (100001, 255, 127, 2, 1), (20011, 1003, 300, 0, 0), (3001, 2047, 65, 5, 5), (18, 1, 3, 0, 0), (40, 2, 1, 0, 0)])
+def test_odd_rows_in_tiles_of_every_size(n, i, o, extra, first):
+    """Rows that start anywhere, through registers: the last piece of the matrix ends with it, what stands between rows is cut off."""
+    gen = torch.Generator().manual_seed(n + i)
+    op, w, b = _linear(gen, i, o, "GELU", bias=True, dtype=torch.bfloat16)
+    whole = torch.full((n, i + extra), float("nan"), dtype=torch.bfloat16, device="cuda")
+    x = whole[:, first:first + i]
+    x.copy_(torch.randn(n, i, generator=gen))
+    y, z = op.forward(x, want_pre_activation=True)
+    ye, ze, error, z_error = ref.linear_forward(x, w, b, None, "GELU")
+    ref.within(y, ye, error, "y")
+    ref.within(z, ze, z_error, "z")
+    dy = _rows(gen, n, o, torch.bfloat16, scale=0.05)
+    dx = op.backward(x, z, dy)
+    e = ref.linear_backward(x, w, z, dy, "GELU")
+    ref.within(dx, *e["dx"], "dx")
+    ref.within(op._grads[:o * i].view(o, i), *e["dw"], "dw")
+    ref.within(op._grads[o * i:], *e["db"], "db")
+
+
 def test_residual_in_place_and_columns_of_one_matrix():
     gen = torch.Generator().manual_seed(4)
     op, w, b = _linear(gen, 64, 64, "SiLU", bias=True, dtype=torch.float16)
