@@ -11,13 +11,13 @@ HALVES = [torch.float16, torch.bfloat16]
 
 
 @pytest.mark.parametrize("dtype", HALVES)
-@pytest.mark.parametrize("kind", ["GELU"])
+@pytest.mark.parametrize("kind", ["GELU", "SiLU"])
 def test_activations_keep_their_tails(kind, dtype):
-    """Every finite value of the type through the epilogue, one layer of a single weight 1: the negative tail is as exact as its own size
-    asks for, down to the smallest numbers of the type.
+    """Every finite value of the type through the epilogue and through the slope, one layer of a single weight 1: the negative tails are as
+    exact as their own size asks for, down to the smallest numbers of the type.
 
-    The bound before the rounding is relative to |y|: 16 half steps of fp32 for what the epilogue computes, and for the exponent -z or
-    -z^2 / 2, formed with at most three roundings, three half steps of it, which is what they move the exponential by."""
+    The bound before the rounding is relative to |y|, or to the two terms of the slope: 16 half steps of fp32 for what is computed, and for
+    the exponent -z or -z^2 / 2, formed with at most three roundings, three half steps of it, which is what they move the exponential by."""
     from neus2_amd.layers import Linear
     values = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
     values = values[torch.isfinite(values)].cuda()[:, None]
@@ -25,6 +25,13 @@ def test_activations_keep_their_tails(kind, dtype):
     op.set_params(torch.ones(1, dtype=dtype, device="cuda"))
     y = op.forward(values)[0]
     z = values.double()
-    exact = z * torch.special.erfc(-z * math.sqrt(0.5)) / 2 if kind == "GELU" else z / (1 + torch.exp(-z))
-    exponent = torch.minimum(z * z / 2 if kind == "GELU" else z.abs(), torch.full_like(z, 200.0))
-    ref.within(y, exact, (16 + 3 * exponent) * ref.U32 * exact.abs(), "y")
+    if kind == "GELU":
+        below, exponent = torch.special.erfc(-z * math.sqrt(0.5)) / 2, z * z / 2
+        second = z * torch.exp(-exponent) / math.sqrt(2 * math.pi)
+    else:
+        below, exponent = torch.exp(torch.minimum(z, torch.zeros_like(z))) / (1 + torch.exp(-z.abs())), z.abs()
+        second = z * below * torch.exp(-torch.maximum(z, torch.zeros_like(z))) / (1 + torch.exp(-z.abs()))
+    relative = (16 + 3 * exponent.clamp(max=200.0)) * ref.U32
+    ref.within(y, z * below, relative * (z * below).abs(), "y")
+    dx = op.backward(values, values, torch.ones_like(values), mode=0)
+    ref.within(dx, below + second, relative * (below + second.abs()), "slope")
