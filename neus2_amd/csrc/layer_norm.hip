@@ -43,10 +43,11 @@ __device__ __forceinline__ void as_loaded(N2Vec<T>& v) {
 	v = __builtin_bit_cast(N2Vec<T>, u);
 }
 
-// sum / width to the last bit, where sum * (1 / width) is a step off: rows of equal values have no variance
+// sum / width to the last bit, where sum * (1 / width) is a step off: rows of equal values have no variance.  (An infinite sum leaves no
+// remainder to correct by.)
 __device__ __forceinline__ float mean_of(float sum, float width, float inv) {
 	const float m = sum * inv;
-	return fmaf(fmaf(-m, width, sum), inv, m);
+	return isinf(m) ? m : fmaf(fmaf(-m, width, sum), inv, m);
 }
 
 // a lane's weights, zero past the width

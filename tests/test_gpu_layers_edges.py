@@ -35,3 +35,21 @@ def test_activations_keep_their_tails(kind, dtype):
     ref.within(y, z * below, relative * (z * below).abs(), "y")
     dx = op.backward(values, values, torch.ones_like(values), mode=0)
     ref.within(dx, below + second, relative * (below + second.abs()), "slope")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width", [8, 12, 1001])
+def test_norm_keeps_an_infinite_mean(width, dtype):
+    """A row with infinities of one sign has that infinity for its mean; the other rows are as without it."""
+    from neus2_amd.layers import LayerNorm
+    gen = torch.Generator().manual_seed(width)
+    x = torch.randn(7, width, generator=gen).to(dtype).cuda()
+    op = LayerNorm(width, dtype=dtype)
+    op.set_params(torch.cat([torch.ones(width), torch.zeros(width)]).to(dtype).cuda())
+    y, (mean, rstd) = op.forward(x, want_ctx=True)
+    x[2, 5], x[4, 0], x[4, 3], x[6, 1], x[6, 2] = math.inf, -math.inf, -math.inf, math.inf, -math.inf
+    y2, (mean2, rstd2) = op.forward(x, want_ctx=True)
+    assert float(mean2[2]) == math.inf and float(mean2[4]) == -math.inf and math.isnan(float(mean2[6]))
+    assert bool(y2[[2, 4, 6]].isnan().all()) and bool(rstd2[[2, 4, 6]].isnan().all())
+    rest = [0, 1, 3, 5]
+    assert torch.equal(y2[rest], y[rest]) and torch.equal(mean2[rest], mean[rest]) and torch.equal(rstd2[rest], rstd[rest])
