@@ -212,6 +212,8 @@ __global__ void __launch_bounds__(threads_of<LANES>(), LANES <= 512u ? 4 : 1) la
 	}
 }
 
+constexpr uint32_t MAX_WIDTH = 16384;
+
 struct Row {
 	uint32_t lanes, chunks;
 };
@@ -225,7 +227,8 @@ Row row_of(uint32_t width, uint32_t vec) {
 	return {0, 0};
 }
 
-template <typename F>
+// f(lanes, vectors) for rows in vectors of VEC values
+template <uint32_t VEC, typename F>
 void with_row(Row row, F&& f) {
 	using std::integral_constant;
 	auto go = [&](auto lanes, auto chunks) { if (row.lanes == lanes() && row.chunks == chunks()) f(lanes, chunks); };
@@ -238,7 +241,7 @@ void with_row(Row row, F&& f) {
 	go(integral_constant<uint32_t, 512>{}, integral_constant<uint32_t, 1>{});
 	go(integral_constant<uint32_t, 1024>{}, integral_constant<uint32_t, 1>{});
 	go(integral_constant<uint32_t, 1024>{}, integral_constant<uint32_t, 2>{});
-	go(integral_constant<uint32_t, 1024>{}, integral_constant<uint32_t, 4>{});
+	if constexpr (1024u * 2u * VEC < MAX_WIDTH) go(integral_constant<uint32_t, 1024>{}, integral_constant<uint32_t, 4>{});
 }
 
 template <typename F>
@@ -249,8 +252,6 @@ void with_types(n2_dtype dtype, n2_dtype weights, F&& f) {
 	if (dtype == N2_DTYPE_BF16 && weights == N2_DTYPE_F32) f(n2_bf16{}, float{});
 	if (dtype == N2_DTYPE_F32) f(float{}, float{});
 }
-
-constexpr uint32_t MAX_WIDTH = 16384;
 
 bool known(n2_dtype t) { return t == N2_DTYPE_F16 || t == N2_DTYPE_BF16 || t == N2_DTYPE_F32; }
 
@@ -275,7 +276,7 @@ N2_API int n2_layer_norm_forward(n2_stream_t stream, n2_dtype dtype, n2_dtype we
 	with_types(dtype, weights_dtype, [&](auto t, auto p) {
 		using T = decltype(t);
 		using P = decltype(p);
-		with_row(row_of(width, N2Vec<T>::SIZE), [&](auto lanes, auto chunks) {
+		with_row<N2Vec<T>::SIZE>(row_of(width, N2Vec<T>::SIZE), [&](auto lanes, auto chunks) {
 			constexpr uint32_t LANES = decltype(lanes)::value, THREADS = threads_of<LANES>(), ROWS = THREADS / LANES;
 			const uint32_t blocks = n2_layer_norm_forward_blocks(n_rows, ROWS, THREADS);
 			layer_norm_forward_kernel<T, P, LANES, decltype(chunks)::value><<<dim3(blocks), dim3(THREADS), 0, n2_stream(stream)>>>(
@@ -290,10 +291,12 @@ N2_API int n2_layer_norm_forward(n2_stream_t stream, n2_dtype dtype, n2_dtype we
 N2_API uint64_t n2_layer_norm_workspace_bytes(n2_dtype dtype, uint32_t n_rows, uint32_t width) {
 	if (!known(dtype) || width < 1 || width > MAX_WIDTH) return 0;
 	uint64_t blocks = 0;
-	with_row(row_of(width, 16u / n2_dtype_bytes(dtype)), [&](auto lanes, auto chunks) {
+	auto count = [&](auto lanes, auto) {
 		constexpr uint32_t LANES = decltype(lanes)::value, THREADS = threads_of<LANES>();
 		blocks = n2_layer_norm_backward_blocks(n_rows, THREADS / LANES, THREADS);
-	});
+	};
+	if (dtype == N2_DTYPE_F32) with_row<4>(row_of(width, 4), count);
+	else with_row<8>(row_of(width, 8), count);
 	return 8ull * width * blocks;
 }
 
@@ -330,7 +333,7 @@ N2_API int n2_layer_norm_backward(n2_stream_t stream, n2_dtype dtype, n2_dtype w
 		with_types(dtype, weights_dtype, [&](auto t, auto p) {
 			using T = decltype(t);
 			using P = decltype(p);
-			with_row(row_of(width, N2Vec<T>::SIZE), [&](auto lanes, auto chunks) {
+			with_row<N2Vec<T>::SIZE>(row_of(width, N2Vec<T>::SIZE), [&](auto lanes, auto chunks) {
 				constexpr uint32_t LANES = decltype(lanes)::value, THREADS = threads_of<LANES>(), ROWS = THREADS / LANES;
 				blocks = n2_layer_norm_backward_blocks(n_rows, ROWS, THREADS);
 				layer_norm_backward_kernel<T, P, LANES, decltype(chunks)::value><<<dim3(blocks), dim3(THREADS), 0, s>>>(
