@@ -2,7 +2,8 @@
 // What bounds it is memory: forward reads a row and writes one, backward reads two (three with a skip connection) and writes one.  A row
 // stays in the registers of the 8 to 1024 lanes that share it, so mean, variance (from the centred values: no cancellation) and result
 // come of one reading.  fp16 on an MI355X: 262 144 x 256 forward 49 us (5.5 TB/s, some of it from the last-level cache; a large copy has 4.8), backward with
-// a skip connection 107 (5.0), 65 536 x 1024 47 and 115 (5.7, 4.7), 2000 x 16 384 32 and 98 (4.1, 2.7: one workgroup to a CU, and sums of 256 rows to join).
+// a skip connection 107 (5.0), 65 536 x 1024 47 and 115 (5.7, 4.7), 2000 x 16 384 33 and 88 (4.0, 3.0: one workgroup to a CU, whose waves load, wait for the
+// row's sums and store together, and sums of 256 rows to join; fp32 52 and 126: 5.0, 4.2).
 #include "column_sums.h"
 
 #include <cmath>
@@ -28,10 +29,14 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*shared)[N]) {
 		__syncthreads();
 #pragma unroll
 		for (uint32_t k = 0; k < N; ++k) {
-			float s = 0.f;
+			if constexpr (WAVES >= 8u) {  // (one value to a lane: sixteen waves' sums of both at once are 32 registers)
+				v[k] = n2_lane_sum<WAVES>(shared[threadIdx.x / LANES * WAVES + threadIdx.x % WAVES][k]);
+			} else {
+				float s = 0.f;
 #pragma unroll
-			for (uint32_t w = 0; w < WAVES; ++w) s += shared[threadIdx.x / LANES * WAVES + w][k];
-			v[k] = s;
+				for (uint32_t w = 0; w < WAVES; ++w) s += shared[threadIdx.x / LANES * WAVES + w][k];
+				v[k] = s;
+			}
 		}
 	}
 }
@@ -129,47 +134,56 @@ __global__ void __launch_bounds__(threads_of<LANES>(), LANES <= 512u ? 4 : 1) la
 	const float inv = 1.f / (float)width;
 	const uint64_t end_x = (uint64_t)(n_rows - 1u) * x_stride + width, end_dy = (uint64_t)(n_rows - 1u) * dy_stride + width, end_skip = (uint64_t)(n_rows - 1u) * skip_stride + width;
 	const Weights<P, LANES, CHUNKS, VEC> w(scale, width, lane);
+	// (four vectors of weights to a lane do not fit beside their gradients' sums: LDS holds them, each lane's own)
+	constexpr bool IN_LDS = CHUNKS > 2u;
+	__shared__ alignas(16) P kept[IN_LDS ? CHUNKS : 1u][LANES][VEC];
+	if constexpr (IN_LDS)
+#pragma unroll
+		for (uint32_t c = 0; c < CHUNKS; ++c) __builtin_memcpy(kept[c][lane], w.v[c], sizeof(w.v[c]));
+	auto weights = [&](uint32_t c) __attribute__((always_inline)) -> const P* { return IN_LDS ? kept[c][lane] : w.v[c]; };
 	float dscale[CHUNKS][VEC] = {}, dshift[CHUNKS][VEC] = {};
 	for (uint64_t first = (uint64_t)blockIdx.x * ROWS; first < n_rows; first += (uint64_t)gridDim.x * ROWS) {
 		const uint64_t row = first + group;
 		const bool live = row < n_rows;
 		const float m = live ? mean[row] : 0.f, s = live ? rstd[row] : 0.f;
-		N2Vec<T> in[CHUNKS], g[CHUNKS], add[CHUNKS];
+		N2Vec<T> in[CHUNKS], g[CHUNKS], early[CHUNKS];
 #pragma unroll
 		for (uint32_t c = 0; c < CHUNKS; ++c) {
 			const uint32_t at = (c * LANES + lane) * VEC, n = live ? n2_left<T>(width, at) : 0u;
 			in[c] = n2_load_row(x, row * x_stride + at, end_x, n);
 			g[c] = n2_load_row(dy, row * dy_stride + at, end_dy, n);
-			add[c] = N2Vec<T>{};
-			if (skip != nullptr) add[c] = n2_load_row(skip, row * skip_stride + at, end_skip, n);
+			early[c] = N2Vec<T>{};  // (of more than one vector the skip connection's come behind the sums: in place too, a lane writes only what it has read)
+			if (CHUNKS == 1u && skip != nullptr) early[c] = n2_load_row(skip, row * skip_stride + at, end_skip, n);
 		}
 		float sum[2] = {0.f, 0.f};
 #pragma unroll
-		for (uint32_t c = 0; c < CHUNKS; ++c)
+		for (uint32_t c = 0; c < CHUNKS; ++c) {
 #pragma unroll
 			for (uint32_t i = 0; i < VEC; ++i) {
-				// (past the width, and for rows past the last, dy is zero and so is the scale)
-				const float xh = ((float)in[c].v[i] - m) * s, d = (float)g[c].v[i], h = d * (float)w.v[c][i];
+				const float xh = ((float)in[c].v[i] - m) * s, d = (float)g[c].v[i], h = d * (float)weights(c)[i];
 				dscale[c][i] += d * xh;
 				dshift[c][i] += d;
 				sum[0] += h;
 				sum[1] += h * xh;
 			}
+		}
 		if (dx == nullptr) continue;
 		row_sums<LANES>(sum, shared);
-		// (the second half takes the rows' values from the registers they came in: kept as fp32 they would halve the waves)
-		if constexpr (LANES <= 256u)
+		// (the second half takes the rows' values from the registers they came in: kept as fp32 they would halve the waves, or not fit)
+		if constexpr (LANES <= 256u || CHUNKS > 1u)
 #pragma unroll
 			for (uint32_t c = 0; c < CHUNKS; ++c) as_loaded(in[c]), as_loaded(g[c]);
 		const float a = sum[0] * inv, b = sum[1] * inv;
 #pragma unroll
 		for (uint32_t c = 0; c < CHUNKS; ++c) {
 			const uint32_t at = (c * LANES + lane) * VEC;
+			N2Vec<T> add = early[c];
+			if (CHUNKS > 1u && skip != nullptr) add = n2_load_row(skip, row * skip_stride + at, end_skip, live ? n2_left<T>(width, at) : 0u);
 			N2Vec<T> out;
 #pragma unroll
 			for (uint32_t i = 0; i < VEC; ++i) {
-				const float xh = ((float)in[c].v[i] - m) * s, h = (float)g[c].v[i] * (float)w.v[c][i];
-				out.v[i] = (T)(s * (h - a - xh * b) + (float)add[c].v[i]);
+				const float xh = ((float)in[c].v[i] - m) * s, h = (float)g[c].v[i] * (float)weights(c)[i];
+				out.v[i] = (T)(s * (h - a - xh * b) + (float)add.v[i]);
 			}
 			n2_store_vec(dx + row * dx_stride + at, out, live ? n2_left<T>(width, at) : 0u);
 		}

@@ -38,6 +38,8 @@ def test_the_linear_layers_sums_stay_in_registers(tmp_path):
 @pytest.mark.skipif(not os.path.exists(build.HIPCC), reason="needs hipcc")
 def test_the_norms_kernels_are_those_that_rows_can_reach(tmp_path):
     """Rows end at 16 384 values: 1024 lanes take them in two vectors of eight, or four of four."""
-    found = [k for k in resources("layer_norm.hip", tmp_path) if "layer_norm_" in k]
+    found = {k: v for k, v in resources("layer_norm.hip", tmp_path).items() if "layer_norm_" in k}
     assert len(found) == 2 * (4 * 9 + 10)
     assert sorted("ffLj1024ELj4E" in k for k in found if "Lj4E" in k) == [True, True]
+    # a row stays in its lanes' registers, the widest too
+    assert not {k: v for k, v in found.items() if v[2] != 0}
