@@ -158,9 +158,12 @@ __global__ void __launch_bounds__(threads_of<LANES>(), LANES <= 512u ? 4 : 1) la
 		float sum[2] = {0.f, 0.f};
 #pragma unroll
 		for (uint32_t c = 0; c < CHUNKS; ++c) {
+			// Past the width, and for rows past the last, dy is zero and so is the scale.  The row's values are zero there, too, and mean * rstd may leave fp32
+			// where no value's own does: equal values, 1e34 with an epsilon of 1e-12.
+			const uint32_t n = n2_left<T>(width, (c * LANES + lane) * VEC);
 #pragma unroll
 			for (uint32_t i = 0; i < VEC; ++i) {
-				const float xh = ((float)in[c].v[i] - m) * s, d = (float)g[c].v[i], h = d * (float)weights(c)[i];
+				const float xh = i < n ? ((float)in[c].v[i] - m) * s : 0.f, d = (float)g[c].v[i], h = d * (float)weights(c)[i];
 				dscale[c][i] += d * xh;
 				dshift[c][i] += d;
 				sum[0] += h;

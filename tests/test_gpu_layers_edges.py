@@ -53,3 +53,24 @@ def test_norm_keeps_an_infinite_mean(width, dtype):
     assert bool(y2[[2, 4, 6]].isnan().all()) and bool(rstd2[[2, 4, 6]].isnan().all())
     rest = [0, 1, 3, 5]
     assert torch.equal(y2[rest], y[rest]) and torch.equal(mean2[rest], mean[rest]) and torch.equal(rstd2[rest], rstd[rest])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width", [1, 12, 63, 1001, 2056, 5000])
+def test_norm_backward_of_equal_values_far_from_zero(width, dtype):
+    """Rows whose mean times 1 / deviation leaves fp32: what stands past the rows' ends in the lanes' vectors has no part in the sums."""
+    from neus2_amd.layers import LayerNorm
+    gen = torch.Generator().manual_seed(width)
+    op = LayerNorm(width, epsilon=1e-12, dtype=dtype)
+    params = torch.cat([1 + 0.1 * torch.randn(width, generator=gen), torch.zeros(width)]).to(dtype).cuda()
+    op.set_params(params, torch.zeros_like(params))
+    x = torch.full((5, width), 1e34, device="cuda").to(dtype)
+    x[1] = torch.randn(width, generator=gen).to(dtype).cuda()
+    dy = torch.randn(5, width, generator=gen).to(dtype).cuda()
+    _, (mean, rstd) = op.forward(x, want_ctx=True)
+    assert bool((rstd[[0, 2, 3, 4]] > 9e5).all())
+    dx = op.backward((mean, rstd), x, dy)
+    e = ref.norm_backward(x, mean, rstd, params[:width], dy, None)
+    ref.within(dx, *e["dx"], "dx")
+    ref.within(op._grads[:width], *e["dscale"], "dscale")
+    ref.within(op._grads[width:], *e["dshift"], "dshift")
