@@ -7,6 +7,7 @@
 #include "layer_types.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <new>
 #include <vector>
@@ -71,11 +72,12 @@ __device__ __forceinline__ double piece_squares(const Piece& p) {
 	return s;
 }
 
+// times factor * 2^exponent
 template <typename T>
-__device__ __forceinline__ void piece_scale(const Piece& p, float factor) {
+__device__ __forceinline__ void piece_scale(const Piece& p, float factor, int exponent) {
 	each_vector<T>(p, [&](N2Vec<T> v, uint32_t at, uint32_t n) __attribute__((always_inline)) {
 #pragma unroll
-		for (uint32_t i = 0; i < N2Vec<T>::SIZE; ++i) v.v[i] = (T)((float)v.v[i] * factor);
+		for (uint32_t i = 0; i < N2Vec<T>::SIZE; ++i) v.v[i] = (T)__builtin_amdgcn_ldexpf((float)v.v[i] * factor, exponent);
 		n2_store_vec(static_cast<T*>(p.out) + at, v, n);
 	});
 }
@@ -120,14 +122,16 @@ __global__ void __launch_bounds__(THREADS) gradient_norm_kernel(const double* __
 __global__ void __launch_bounds__(THREADS) gradient_clip_kernel(const Piece* __restrict__ pieces, uint32_t n_pieces, const double* __restrict__ partial, uint32_t n_partial, float max_norm,
                                                                 float loss_scale, float* __restrict__ norm) {
 	const double n = norm_of(partial, n_partial, (double)loss_scale), ratio = (double)max_norm / (n + 1e-6);
-	const float factor = ratio > 1. ? 1.f : (float)ratio;  // (no number stays none)
+	float factor = ratio > 1. ? 1.f : (float)ratio;  // (no number stays none)
+	int exponent = 0;
+	if (factor < FLT_MIN && ratio > 0.) factor = (float)frexp(ratio, &exponent);  // (no normal number of fp32, where its products may be)
 	if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
 	for (uint32_t i = blockIdx.x; i < n_pieces; i += gridDim.x) {
 		const Piece p = pieces[n_pieces - 1u - i];
 		if (p.in == p.out && factor == 1.f) continue;
-		if (p.dtype == N2_DTYPE_F16) piece_scale<n2_f16>(p, factor);
-		else if (p.dtype == N2_DTYPE_BF16) piece_scale<n2_bf16>(p, factor);
-		else piece_scale<float>(p, factor);
+		if (p.dtype == N2_DTYPE_F16) piece_scale<n2_f16>(p, factor, exponent);
+		else if (p.dtype == N2_DTYPE_BF16) piece_scale<n2_bf16>(p, factor, exponent);
+		else piece_scale<float>(p, factor, exponent);
 	}
 }
 

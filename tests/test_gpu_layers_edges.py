@@ -74,3 +74,19 @@ def test_norm_backward_of_equal_values_far_from_zero(width, dtype):
     ref.within(dx, *e["dx"], "dx")
     ref.within(op._grads[:width], *e["dscale"], "dscale")
     ref.within(op._grads[width:], *e["dshift"], "dshift")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size,loss_scale,max_norm", [(1e19, 1e-25, 1.0), (1e30, 1e-30, 0.5), (1e5, 1.0, 1e-39), (3e37, 1.0, 1e-2)])
+def test_clip_by_a_factor_below_fp32(size, loss_scale, max_norm, dtype):
+    """max_norm / norm is no normal number of fp32, or zero, where the clipped gradients are: bound, half a step for the factor in fp64 and the product each."""
+    from neus2_amd.layers import GradientClip
+    gen = torch.Generator().manual_seed(3)
+    g = (torch.randn(5003, generator=gen) * size).to(dtype).cuda()
+    before = g.double()
+    norm = float(before.square().sum().sqrt()) / torch.tensor(loss_scale, dtype=torch.float32).double().item()
+    factor = torch.tensor(max_norm, dtype=torch.float32).double().item() / (norm + 1e-6)
+    assert factor < 1.2e-38
+    GradientClip([g]).clip(max_norm, loss_scale=loss_scale)
+    exact = before * factor
+    ref.within(g, exact, 4 * ref.U32 * exact.abs(), "clipped")
