@@ -29,20 +29,12 @@ constexpr uint32_t THREADS = 256, MAX_BLOCKS = N2_GRADIENTS_WORKSPACE_BYTES / si
 constexpr uint64_t PIECE_STEP = THREADS * 16, MOST_STEPS = 16;
 
 // Squares are summed in fp64: those of fp32 and bf16 leave fp32's range long before the values do.
-// (Those of fp16 are exact in fp32, and eight of them lie well inside its range.)
 template <typename T>
 __device__ __forceinline__ double squares(const N2Vec<T>& v) {
 	double s = 0.;
 #pragma unroll
 	for (uint32_t i = 0; i < N2Vec<T>::SIZE; ++i) s = fma((double)(float)v.v[i], (double)(float)v.v[i], s);
 	return s;
-}
-template <>
-__device__ __forceinline__ double squares<n2_f16>(const N2Vec<n2_f16>& v) {
-	float s = 0.f;
-#pragma unroll
-	for (uint32_t i = 0; i < 8u; ++i) s = fmaf((float)v.v[i], (float)v.v[i], s);
-	return (double)s;
 }
 
 // f(vector, place, valid values) for a lane's vectors of a piece, four loads under way at a time.  (The norm with two, four and eight, us: 40

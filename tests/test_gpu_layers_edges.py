@@ -90,3 +90,14 @@ def test_clip_by_a_factor_below_fp32(size, loss_scale, max_norm, dtype):
     GradientClip([g]).clip(max_norm, loss_scale=loss_scale)
     exact = before * factor
     ref.within(g, exact, 4 * ref.U32 * exact.abs(), "clipped")
+
+
+def test_the_norm_of_fp16_gradients_loses_no_small_square():
+    """Squares of 10.5 beside those of 60 000, a step of fp32 for 256: the sum is fp64's, so the norm is off by its own rounding alone (and 2^-40 for the sum's)."""
+    from neus2_amd.layers import GradientClip
+    g = torch.full((4096, 8), 10.5, dtype=torch.float16, device="cuda")
+    g[:, 3] = 60000.0
+    exact = math.sqrt(float(g.double().square().sum()))
+    clip = GradientClip([g], out=[torch.empty_like(g)])
+    for norm in (clip.norm(), clip.clip(1.0)):
+        assert abs(float(norm) - exact) <= (ref.U32 + 2.0 ** -40) * exact
