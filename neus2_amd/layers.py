@@ -243,7 +243,8 @@ class GradientClip:
     """The norm over the gradients of many tensors, and their scaling to at most a given norm, in front of an optimiser's step.
 
     gradients: tensors without gaps, fp16, bf16 and fp32 in any mixture, that do not overlap (kept alive here: every call reads what
-    they hold then).  out: tensors of the same types and sizes for the clipped gradients; None clips in place."""
+    they hold then).  out: tensors of the same types and sizes for the clipped gradients; None clips in place.  The table of the tensors'
+    addresses is this object's: calls on any stream may be under way when it is dropped, but a captured graph needs it alive."""
 
     def __init__(self, gradients, out=None):
         gradients = list(gradients)
@@ -263,8 +264,9 @@ class GradientClip:
         nbytes = L.n2_gradients_table_bytes(len(gradients), tensors)
         self._keep = (gradients, out)
         self._table = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+        self._stream = _stream_of(_current_device())
         self._h = C.c_void_p()
-        check(L.n2_gradients_create(_stream_address(), len(gradients), tensors, self._table.data_ptr(), nbytes, C.byref(self._h)), "n2_gradients_create")
+        check(L.n2_gradients_create(self._stream, len(gradients), tensors, self._table.data_ptr(), nbytes, C.byref(self._h)), "n2_gradients_create")
 
     def __del__(self):
         try:
@@ -276,18 +278,20 @@ class GradientClip:
 
     def _buffers(self):
         table = self._table
-        device = _check_device(table, "the gradients' table")
-        return device, table.new_empty((), dtype=torch.float32), table.new_empty(capi.GRADIENTS_WORKSPACE_BYTES)
+        stream = _stream_of(_check_device(table, "the gradients' table"))
+        if stream != self._stream:  # (the table's memory goes to nobody else before this stream has read it)
+            table.record_stream(torch.cuda.current_stream())
+        return stream, table.new_empty((), dtype=torch.float32), table.new_empty(capi.GRADIENTS_WORKSPACE_BYTES)
 
     def norm(self, loss_scale=1.0):
         """sqrt(sum of squares) / loss_scale as a one-element device tensor (no host synchronisation)."""
-        device, norm, ws = self._buffers()
-        check(capi.lib().n2_gradients_norm(self._h, _stream_of(device), loss_scale, norm.data_ptr(), ws.data_ptr(), capi.GRADIENTS_WORKSPACE_BYTES), "n2_gradients_norm")
+        stream, norm, ws = self._buffers()
+        check(capi.lib().n2_gradients_norm(self._h, stream, loss_scale, norm.data_ptr(), ws.data_ptr(), capi.GRADIENTS_WORKSPACE_BYTES), "n2_gradients_norm")
         return norm
 
     def clip(self, max_norm, loss_scale=1.0):
         """Multiplies the gradients by min(1, max_norm / (norm + 1e-6)); they keep their loss scale (Adam.step's, whose gradients
         are loss_scale times the loss's).  Returns the norm before, as norm() does."""
-        device, norm, ws = self._buffers()
-        check(capi.lib().n2_gradients_clip(self._h, _stream_of(device), max_norm, loss_scale, norm.data_ptr(), ws.data_ptr(), capi.GRADIENTS_WORKSPACE_BYTES), "n2_gradients_clip")
+        stream, norm, ws = self._buffers()
+        check(capi.lib().n2_gradients_clip(self._h, stream, max_norm, loss_scale, norm.data_ptr(), ws.data_ptr(), capi.GRADIENTS_WORKSPACE_BYTES), "n2_gradients_clip")
         return norm

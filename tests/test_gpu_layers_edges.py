@@ -101,3 +101,27 @@ def test_the_norm_of_fp16_gradients_loses_no_small_square():
     clip = GradientClip([g], out=[torch.empty_like(g)])
     for norm in (clip.norm(), clip.clip(1.0)):
         assert abs(float(norm) - exact) <= (ref.U32 + 2.0 ** -40) * exact
+
+
+def test_a_dropped_clips_table_waits_for_the_streams_that_read_it():
+    """The table is made on one stream and read on another, where the call waits behind a long piece of work: dropped then, its memory is not
+    handed out again before that call is done, and the clipped gradients are right."""
+    from neus2_amd.layers import GradientClip
+    tensors = [torch.full((64,), 1.0, device="cuda") for _ in range(2000)]
+    big = torch.ones(1 << 28, device="cuda")
+    side = torch.cuda.Stream()
+    clip = GradientClip(tensors)
+    table, size = clip._table.data_ptr(), clip._table.numel()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(200):
+            big.mul_(1.0)
+        norm = clip.clip(1.0)
+        done = side.record_event()
+    del clip
+    new = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    early = not done.query()
+    assert early and all(t.data_ptr() != table for t in new)
+    torch.cuda.synchronize()
+    assert float(norm) == pytest.approx(math.sqrt(128000.0), rel=1e-6)
+    assert all(float(t[0]) == pytest.approx(1 / math.sqrt(128000.0), rel=1e-5) for t in tensors[::100])
