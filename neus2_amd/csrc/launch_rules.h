@@ -344,6 +344,12 @@ static inline N2LinearPlan n2_linear_plan(uint32_t m, uint32_t n, uint32_t k) {
 }
 static inline uint64_t n2_linear_partial_bytes(const N2LinearPlan& plan, uint32_t m, uint32_t n) { return plan.splits > 1 ? 4ull * plan.splits * m * n : 0ull; }
 
+// Rows of C to one launch of a product in tiles whose splits are `splits` (more than one only where tiles are few): the threads of a launch are counted in 32 bits.
+static inline uint32_t n2_linear_launch_rows(uint32_t m, uint32_t tile, uint32_t tiles_n, uint32_t splits) {
+	const uint32_t threads = tile == 256u ? 512u : 256u, most = 0xFFFFFFFFu / threads / (tiles_n * splits);
+	return n2_ceil_div(m, tile) <= most ? m : most * tile;
+}
+
 // Whether a forward pass has so few rows that its weights go straight into registers (few_rows_kernel).  GPU time in us, that way | in tiles:
 // 1 x 2048 x 2048 4.5 | 7.2, 8 x 4000 x 300 6.5 | 8.2, 16 x 2048 x 2048 5.9 | 8.7, 16 x 4096 x 4096 10.1 | 11.5, 16 x 333 x 77 4.9 | 10.4; two and four
 // instructions of rows 32 x 1024 x 1024 5.9 | 5.8, 32 x 4096 x 4096 13.9 | 11.4, 64 x 2048 x 2048 11.4 | 9.2, 64 x 4000 x 64 14.8 | 7.9.

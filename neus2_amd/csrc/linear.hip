@@ -817,23 +817,37 @@ void plan_product(Product& q, const N2LinearPlan& plan, float* partial) {
 uint64_t blocks_of(const Product& q) { return (uint64_t)q.tiles_m * q.tiles_n * q.splits; }
 
 template <typename T, bool A_KC, bool B_KC, int EPI>
-int launch_product(hipStream_t s, const Product& q, uint32_t tile) {
-	N2_REQUIRE(blocks_of(q) <= 0xFFFFFFFFull / 512u, "n2_linear: %u x %u values take %llu workgroups", q.m, q.n, (unsigned long long)blocks_of(q));
-	const dim3 grid((uint32_t)blocks_of(q));
-	auto launch = [&](auto async, auto out) {
-		constexpr bool ASYNC = decltype(async)::value;
-		constexpr int OUT = decltype(out)::value;
-		if (tile == 256) product_kernel<T, ASYNC, A_KC, B_KC, 256, 2, 4, EPI, OUT><<<grid, dim3(512), 0, s>>>(q);
-		else if (tile == 128) product_kernel<T, ASYNC, A_KC, B_KC, 128, 2, 2, EPI, OUT><<<grid, dim3(256), 0, s>>>(q);
-		else product_kernel<T, ASYNC, A_KC, B_KC, 64, 2, 2, EPI, OUT><<<grid, dim3(256), 0, s>>>(q);
+int launch_product(hipStream_t s, const Product& all, uint32_t tile) {
+	const auto launch_rows = [&](const Product& q) -> int {
+		const dim3 grid((uint32_t)blocks_of(q));
+		auto launch = [&](auto async, auto out) {
+			constexpr bool ASYNC = decltype(async)::value;
+			constexpr int OUT = decltype(out)::value;
+			if (tile == 256) product_kernel<T, ASYNC, A_KC, B_KC, 256, 2, 4, EPI, OUT><<<grid, dim3(512), 0, s>>>(q);
+			else if (tile == 128) product_kernel<T, ASYNC, A_KC, B_KC, 128, 2, 2, EPI, OUT><<<grid, dim3(256), 0, s>>>(q);
+			else product_kernel<T, ASYNC, A_KC, B_KC, 64, 2, 2, EPI, OUT><<<grid, dim3(256), 0, s>>>(q);
+		};
+		auto with_out = [&](auto async) {
+			if (q.partial != nullptr) launch(async, std::integral_constant<int, SPLIT>{});
+			else launch(async, std::integral_constant<int, WHOLE>{});
+		};
+		if (async_product<A_KC, B_KC>(q)) with_out(std::true_type{});
+		else with_out(std::false_type{});
+		N2_LAUNCH_CHECK();
+		return N2_OK;
 	};
-	auto with_out = [&](auto async) {
-		if (q.partial != nullptr) launch(async, std::integral_constant<int, SPLIT>{});
-		else launch(async, std::integral_constant<int, WHOLE>{});
-	};
-	if (async_product<A_KC, B_KC>(q)) with_out(std::true_type{});
-	else with_out(std::false_type{});
-	N2_LAUNCH_CHECK();
+	// (where C's rows are widths, at most 65 536 of them, one launch takes all)
+	const uint32_t most = A_KC ? n2_linear_launch_rows(all.m, tile, all.tiles_n, all.splits) : all.m;
+	if (most >= all.m) return launch_rows(all);
+	for (uint64_t first = 0; first < all.m; first += most) {
+		Product q = all;
+		q.m = q.extent_a = (uint32_t)(all.m - first < most ? all.m - first : most);
+		q.tiles_m = n2_ceil_div(q.m, tile);
+		q.a.p = static_cast<const T*>(all.a.p) + first * all.a.ld, q.c = static_cast<T*>(all.c) + first * all.ldc;
+		if (all.residual != nullptr) q.residual = static_cast<const T*>(all.residual) + first * all.ldr;
+		if (all.pre != nullptr) q.pre = static_cast<T*>(all.pre) + first * all.ldp;
+		if (const int rc = launch_rows(q)) return rc;
+	}
 	return N2_OK;
 }
 
@@ -1041,7 +1055,7 @@ N2_API int n2_linear_backward(n2_stream_t stream, n2_dtype dtype, n2_activation 
 			plan_product(w, p.weights, partial + p.input_partial);
 		}
 		const bool async = async_product<true, false>(x);
-		if (has_x && !streams && dw != nullptr && small && async == async_product<false, false>(w) && blocks_of(x) + blocks_of(w) <= 0xFFFFFFFFull / 512u) {
+		if (has_x && !streams && dw != nullptr && small && async == async_product<false, false>(w) && blocks_of(x) + blocks_of(w) <= 0xFFFFFFFFull / 256u) {
 			const dim3 grid((uint32_t)(blocks_of(x) + blocks_of(w)));
 			if (async) product_pair_kernel<T, true><<<grid, dim3(256), 0, s>>>(x, w, (uint32_t)blocks_of(x));
 			else product_pair_kernel<T, false><<<grid, dim3(256), 0, s>>>(x, w, (uint32_t)blocks_of(x));

@@ -125,3 +125,28 @@ def test_a_dropped_clips_table_waits_for_the_streams_that_read_it():
     torch.cuda.synchronize()
     assert float(norm) == pytest.approx(math.sqrt(128000.0), rel=1e-6)
     assert all(float(t[0]) == pytest.approx(1 / math.sqrt(128000.0), rel=1e-5) for t in tensors[::100])
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_as_many_rows_as_there_can_be(residual):
+    """2^31 - 1 rows of one value, in tiles: more workgroups than one launch has threads for.  Every value is checked: all are small whole
+    numbers, exact in fp16 but for the weight's gradient, which is rounded once."""
+    from neus2_amd.layers import Linear
+    n = (1 << 31) - 1
+    op = Linear(1, 1, activation="ReLU", dtype=torch.float16)
+    params = torch.tensor([2.0, -8.0], dtype=torch.float16, device="cuda")
+    op.set_params(params, torch.zeros_like(params))
+    x = torch.arange(13, dtype=torch.float16, device="cuda").repeat(n // 13 + 1)[:n, None]
+    y, z = op.forward(x, residual=x if residual else None, want_pre_activation=True)
+    assert torch.equal(z, x * 2 - 8)
+    assert torch.equal(y, z.clamp(min=0) + x if residual else z.clamp(min=0))
+    if residual:
+        return
+    del y
+    dy = torch.zeros_like(x)
+    dy[::1 << 20] = 1.0  # 2048 rows of a gradient
+    dy[-5:] = 1.0
+    dx = op.backward(x, z, dy)
+    on = (z > 0) & (dy > 0)
+    assert torch.equal(dx, on.half() * 2)
+    assert float(op._grads[0]) == float(torch.tensor(float(x[on].double().sum())).half()) and float(op._grads[1]) == float(torch.tensor(float(on.sum())).half())
