@@ -150,3 +150,31 @@ def test_as_many_rows_as_there_can_be(residual):
     on = (z > 0) & (dy > 0)
     assert torch.equal(dx, on.half() * 2)
     assert float(op._grads[0]) == float(torch.tensor(float(x[on].double().sum())).half()) and float(op._grads[1]) == float(torch.tensor(float(on.sum())).half())
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("kind", ["SiLU", "GELU"])
+@pytest.mark.parametrize("n,i,o", [(5, 24, 40), (300, 72, 96), (5003, 320, 257), (3000, 264, 520), (50000, 64, 128), (49155, 200, 72)])
+def test_the_backward_pass_rounds_dz_once(n, i, o, kind, dtype):
+    """dL/dz meets the matrix cores in the layer's type, the one rounding besides the results' own: with the identity for weights the input's
+    gradient is dL/dz as it was rounded, and from that the gradients of any weights are off by their fp32 sums and their own rounding alone."""
+    from neus2_amd.layers import Linear
+    gen = torch.Generator().manual_seed(n + i)
+    z, dy = (torch.randn(n, o, generator=gen).to(dtype).cuda() for _ in range(2))
+    x = torch.randn(n, i, generator=gen).to(dtype).cuda()
+    identity = Linear(o, o, activation=kind, bias=False, dtype=dtype)
+    identity.set_params(torch.eye(o, dtype=dtype, device="cuda").reshape(-1))
+    dz = identity.backward(torch.zeros(n, o, dtype=dtype, device="cuda"), z, dy, mode=0)
+    g = dy.double()
+    ref.within(dz, g * ref.slope(z.double(), kind), 2.0 ** -20 * g.abs(), "dz")
+    op = Linear(i, o, activation=kind, dtype=dtype)
+    w = (torch.randn(o, i, generator=gen) / math.sqrt(o)).to(dtype).cuda()
+    params = torch.cat([w.reshape(-1), torch.zeros(o, dtype=dtype, device="cuda")])
+    op.set_params(params, torch.zeros_like(params))
+    dx = op.backward(x, z, dy)
+    d = dz.double()
+    ref.within(dx, d @ w.double(), 2 * (o + 2) * ref.U32 * (d.abs() @ w.double().abs()), "dx")
+    ref.within(op._grads[:o * i].view(o, i), d.T @ x.double(), 2 * (n + 66) * ref.U32 * (d.abs().T @ x.double().abs()), "dw")
+    if n > 40000:
+        dx = op.backward(x, z, dy, mode=0)  # (formed on the way to dx)
+        ref.within(dx, d @ w.double(), 2 * (o + 2) * ref.U32 * (d.abs() @ w.double().abs()), "dx alone")
