@@ -990,7 +990,7 @@ int n2_layer_norm_backward(n2_stream_t stream, n2_dtype dtype, n2_dtype weights_
  *   norm = sqrt(sum of squares of all gradients) / loss_scale, summed in fp64: no square overflows or vanishes
  *   factor = min(1, max_norm / (norm + 1e-6)); out = gradient * factor (loss_scale stays in them)
  * A norm that is no number makes every gradient one; an infinite one makes finite gradients zero and infinite ones no
- * numbers.  In place and with a factor of 1 nothing is written. */
+ * numbers (all of them, where max_norm is infinite too).  In place and with a factor of 1 nothing is written. */
 typedef struct n2_gradients n2_gradients_t;
 typedef struct n2_gradient_tensor {
 	const void* d_gradients; /* n values of dtype, without gaps */

@@ -2,8 +2,8 @@
 // What bounds it is memory: forward reads a row and writes one, backward reads two (three with a skip connection) and writes one.  A row
 // stays in the registers of the 8 to 1024 lanes that share it, so mean, variance (from the centred values: no cancellation) and result
 // come of one reading.  fp16 on an MI355X: 262 144 x 256 forward 49 us (5.5 TB/s, some of it from the last-level cache; a large copy has 4.8), backward with
-// a skip connection 107 (5.0), 65 536 x 1024 47 and 115 (5.7, 4.7), 2000 x 16 384 33 and 88 (4.0, 3.0: one workgroup to a CU, whose waves load, wait for the
-// row's sums and store together, and sums of 256 rows to join; fp32 52 and 126: 5.0, 4.2).
+// a skip connection 107 (5.0), 65 536 x 1024 47 and 115 (5.7, 4.7), 2000 x 16 384 33 and 89 (4.0, 2.9: one workgroup to a CU, whose waves load, wait for the
+// row's sums and store together, and sums of 256 rows to join; fp32 52 and 127: 5.0, 4.1).
 #include "column_sums.h"
 
 #include <cmath>

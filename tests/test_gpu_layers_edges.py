@@ -178,3 +178,12 @@ def test_the_backward_pass_rounds_dz_once(n, i, o, kind, dtype):
     if n > 40000:
         dx = op.backward(x, z, dy, mode=0)  # (formed on the way to dx)
         ref.within(dx, d @ w.double(), 2 * (o + 2) * ref.U32 * (d.abs() @ w.double().abs()), "dx alone")
+
+
+def test_an_infinite_limit_clips_nothing():
+    from neus2_amd.layers import GradientClip
+    g = torch.arange(1.0, 101.0, device="cuda")
+    clip = GradientClip([g])
+    assert float(clip.clip(math.inf)) == pytest.approx(math.sqrt(338350.0), rel=2 * ref.U32) and torch.equal(g, torch.arange(1.0, 101.0, device="cuda"))
+    g[7] = math.inf
+    assert float(clip.clip(math.inf)) == math.inf and bool(g.isnan().all())
