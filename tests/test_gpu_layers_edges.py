@@ -187,3 +187,27 @@ def test_an_infinite_limit_clips_nothing():
     assert float(clip.clip(math.inf)) == pytest.approx(math.sqrt(338350.0), rel=2 * ref.U32) and torch.equal(g, torch.arange(1.0, 101.0, device="cuda"))
     g[7] = math.inf
     assert float(clip.clip(math.inf)) == math.inf and bool(g.isnan().all())
+
+
+def test_a_captured_clip_replays_and_is_dropped():
+    """Made on one stream, captured on another: every replay clips what the tensors hold then, as eager calls do, and the object goes behind its graph."""
+    from neus2_amd.layers import GradientClip
+    gen = torch.Generator().manual_seed(4)
+    sizes = [70000, 333, 1]
+    g = [torch.zeros(k, device="cuda") for k in sizes]
+    clip = GradientClip(g)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = clip.clip(0.5, loss_scale=2.0)
+    for _ in range(4):
+        fresh = [torch.randn(k, generator=gen).cuda() for k in sizes]
+        [t.copy_(f) for t, f in zip(g, fresh)]
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed, n = [t.clone() for t in g], norm.clone()
+        [t.copy_(f) for t, f in zip(g, fresh)]
+        assert torch.equal(clip.clip(0.5, loss_scale=2.0), n) and all(torch.equal(a, b) for a, b in zip(g, replayed))
+    del graph
+    del clip
+    torch.cuda.synchronize()
+    assert float(GradientClip(g).norm()) == pytest.approx(1.0, rel=1e-5)
